@@ -9,7 +9,7 @@ declare -A built
 for spec in "$@"; do
   src=${spec%%=*}; flags=${spec#*=}; flags=${flags//,/ }
   obj=$out/${src%.hip}.o
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -fPIC -std=c++17 -munsafe-fp-atomics -Wno-unused-result -DTF_EXPERIMENTS $flags -c transfusion_amd/csrc/$src -o $obj
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -fPIC -std=c++17 -munsafe-fp-atomics -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops -DTF_EXPERIMENTS $flags -c transfusion_amd/csrc/$src -o $obj
   built[${src%.hip}]=$obj
 done
 objs=""

@@ -463,9 +463,11 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dkv_x3_kernel(const TfAttnArg
     r_dw = a.drop_thr ? (in ? dbits[(size_t)q * dw_ld] : 0u) : 0xffffffffu;
     r_bw = blk ? bbits[(size_t)q * dw_ld] : 0u;
   };
+  // (the dK launch at head dim 224 fills the register file: its scalars are read in place, the four registers would spill)
+  constexpr bool AHEAD = !(WHICH == 1 && HDP > 192);
   float n_lse = 0.f, n_del = 0.f;
   unsigned n_dw = 0u, n_bw = 0u;
-  if (ntiles > 0) row_scalars(0, n_lse, n_del, n_dw, n_bw);
+  if (AHEAD && ntiles > 0) row_scalars(0, n_lse, n_del, n_dw, n_bw);
   // DEFER (the dK launch that stores dS / Pd tiles, head dims <= 192): the 8 tile stores of tile t are ISSUED at the start of tile
   // t + 1's matrix phase.  vmcnt retires in issue order, so the staging wait of the next tile (global loads -> LDS) also waits for
   // every older store: issued right behind the softmax they had only the 36 MFMAs of the dK product to complete in, and the wait
@@ -493,9 +495,10 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dkv_x3_kernel(const TfAttnArg
     const int q0 = t * 32;
     __syncthreads();
     stage_quad<32, HDP>(q_h, q_l, ldq, false, qt_h, qt_l, do_h, do_l, a.ld_dout, true, dot_h, dot_l, q0, Sqb - 1, tid);   // dO rows >= Sqb: zero
+    if (!AHEAD) row_scalars(q0, n_lse, n_del, n_dw, n_bw);
     if (tid < 32) { lse_s[tid] = n_lse; del_s[tid] = n_del; }
     if (lane < 32) { dw_s[wave * 32 + lane] = n_dw; bw_s[wave * 32 + lane] = n_bw; }
-    if (t + 1 < ntiles) row_scalars(q0 + 32, n_lse, n_del, n_dw, n_bw);
+    if (AHEAD && t + 1 < ntiles) row_scalars(q0 + 32, n_lse, n_del, n_dw, n_bw);
     __syncthreads();
     f32x16 st, dp;
 #pragma unroll
