@@ -23,7 +23,7 @@ extern "C" {
 #endif
 
 typedef void* tf_stream_t;   /* hipStream_t */
-#define TF_ABI_VERSION 10
+#define TF_ABI_VERSION 11
 #define TF_MAX_LAYERS 16
 #define TF_MAX_GROUPS 8     /* ragged groups (ABI v8): at most this many row ranges of unequal size in one grouped launch */
 
@@ -593,6 +593,63 @@ int tf_allreduce_bucket(TfComm* comm, float* buf, long long n, tf_stream_t s);  
 /* collectives issued / fp32 elements reduced so far on this rank (all ranks must agree); any out pointer may be null */
 int tf_comm_stats(const TfComm* comm, int* world, int* rank, long long* calls, long long* elems);
 int tf_comm_destroy(TfComm* comm);
+
+/* ---- positions and score-modified attention, norm over many tensors (ABI v11; no reference counterpart) ----------------------
+ * Rotary positions with several axes: channel pair p of every head turns by pos[token][axis[p]] * base frequency, (a, b) ->
+ * (a cos - b sin, a sin + b cos).  Pairs are channels (p, pairs + p), or (2p, 2p + 1) when interleaved; channels from 2 * pairs on pass
+ * through.  inverse != 0 turns back (the gradient).  Q and K in one launch; either may have no heads.  Angles are formed in 64 bits. */
+typedef struct TfRotaryArgs {
+  const void* q; long long q_sb, q_ss, q_sh;     // [B, S, H, D], strides of batch, token and head in ELEMENTS, channels contiguous
+  const void* k; long long k_sb, k_ss, k_sh;     // [B, S, Hk, D]
+  void* q_out; void* k_out;                      // contiguous [B, S, H, D] / [B, S, Hk, D]; no overlap with the inputs
+  int B, S, H, Hk, D; int is_f32;                // bf16 or fp32
+  const void* pos; int pos_type;                 // [B, S, n_axes] (pos_batched) or [S, n_axes], contiguous; 0 int32, 1 int64, 2 fp32
+  int pos_batched; int n_axes;
+  const double* inv_freq;                        // [pairs] device: radians per position step DIVIDED BY 2 pi
+  const int* axis;                               // [pairs] device: axis of the pair, in [0, n_axes)
+  int pairs; int interleaved; int inverse;
+} TfRotaryArgs;
+int tf_rotary(const TfRotaryArgs* a, tf_stream_t s);
+
+/* Attention with changed scores, forward and backward.  For query i of sample b at position p = q_start[b] + i (default Sk - Sq + i) and
+ * key j:  s = scale q.k;  softcap > 0: s = softcap tanh(s / softcap);  s -= slopes[h] |p - j|;  the key is hidden unless
+ * q_doc[b][i] == k_doc[b][j] >= 0 (when given) and (causal == 0 or j <= p or j < prefix[b]).  Rows without keys give zeros and take no
+ * gradient.  What rows of negative documents, and keys beyond the causal horizon of the last query, hold in memory is never used (NaN
+ * included).  H % Hk == 0: H / Hk consecutive heads share a key / value head.  D <= 256, D % 8 == 0; bf16 or fp32; every
+ * pointer and stride a multiple of 16 bytes.  Statistics and sums are fp32; results do not depend on the launch's timing. */
+typedef struct TfScoreAttnArgs {
+  const void* q; long long q_sb, q_ss, q_sh;     // [B, Sq, H, D], strides of batch, token and head in elements, channels contiguous
+  const void* k; long long k_sb, k_ss, k_sh;     // [B, Sk, Hk, D]
+  const void* v; long long v_sb, v_ss, v_sh;     // [B, Sk, Hk, D]
+  void* out;                                     // [B, Sq, H, D] contiguous
+  float* lse;                                    // [B, H, Sq] fp32 (log2 domain; +inf for rows without keys), or null without a backward
+  int B, Sq, Sk, H, Hk, D; int is_f32;
+  float scale, softcap;
+  const float* slopes;                           // [H] fp32 or null
+  int causal; const int* prefix; const int* q_start;   // [B] int32 device arrays or null
+  const int* q_doc; const int* k_doc;            // [B, Sq] / [B, Sk] int32 contiguous, both or neither
+  void* work; size_t work_bytes;                 // forward: tf_score_attn_work(a) bytes (0: none needed)
+  // backward (lse from the forward)
+  const void* dout; long long do_sb, do_ss, do_sh;   // [B, Sq, H, D]
+  void* dq; void* dk; void* dv;                  // contiguous, layouts of q / k / v
+  float* delta;                                  // [B, H, Sq] fp32 workspace
+  float* dslopes; float* dslope_rows;            // [H] out and [B, H, Sq] workspace, or both null
+} TfScoreAttnArgs;
+size_t tf_score_attn_work(const TfScoreAttnArgs* a);
+int tf_score_attn_fwd(const TfScoreAttnArgs* a, tf_stream_t s);
+int tf_score_attn_bwd(const TfScoreAttnArgs* a, tf_stream_t s);
+
+/* Norm over many tensors and clipping: norm[0] = sqrt(sum g^2) (norm_type 0) or max |g| (1, NaN wins); clip != 0: g *= min(1, max_norm /
+ * (norm + 1e-6)), rounded once to the tensor's type.  The three arrays are HOST memory, read before the call returns.  No two tensors may
+ * overlap.  Deterministic: partial sums in 64 bits, added in one order. */
+typedef struct TfGradClipArgs {
+  void** grads; const long long* n; const int* is_bf16;   // [count] device pointers, element counts, types (0 fp32, 1 bf16)
+  int count; int norm_type; int clip; float max_norm;
+  float* norm;                                   // [1] device
+  void* work; long long parts;                   // workspace of parts doubles; parts >= tf_grad_clip_parts(n, count)
+} TfGradClipArgs;
+long long tf_grad_clip_parts(const long long* n, int count);     // < 0: lengths out of range
+int tf_grad_clip(const TfGradClipArgs* a, tf_stream_t s);
 
 /* ---- launch tracer (measurement only) ----
  * Between tf_trace_start and tf_trace_stop every kernel launch of this library is bracketed by a HIP event pair on

@@ -134,6 +134,10 @@ def load():
     lib.tf_trace_stop.argtypes = [C.c_void_p, C.c_longlong]
     for f in ("tf_sumsq", "tf_sumsq_set"):
         getattr(lib, f).argtypes = [C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p]
+    lib.tf_score_attn_work.restype = C.c_size_t
+    lib.tf_score_attn_work.argtypes = [C.c_void_p]
+    lib.tf_grad_clip_parts.restype = C.c_longlong
+    lib.tf_grad_clip_parts.argtypes = [C.c_void_p, C.c_int]
     lib.tf_dropout_mask.argtypes = [C.c_void_p, C.c_longlong, C.c_uint32, C.c_uint32, C.c_void_p]
     lib.tf_dropout_apply.argtypes = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_uint32, C.c_uint32, C.c_float, C.c_void_p]
     lib.tf_cast_f32_bf16.argtypes = [C.c_void_p, C.c_void_p, C.c_longlong, C.c_void_p]

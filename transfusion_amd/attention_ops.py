@@ -1,0 +1,265 @@
+"""Rotary positions with several axes and attention with changed scores (capped, biased by distance, masked by documents, a causal
+horizon and a bidirectional prefix), over the C ABI (``tf_rotary``, ``tf_score_attn_*``; include/tfusion.h).  bf16 or fp32 tensors
+[B, tokens, heads, head_dim] of any batch / token / head strides: the thirds of a packed projection go in as they are.  Both run under
+autograd, on the current stream of their tensors' device; CPU tensors raise -- there is no CPU path.
+
+    plan = RotaryPlan(192, axes=(32, 32, 32), device=dev)             # time, height, width: 32 channel pairs each
+    q, k = rotary(q, k, pos, plan)                                    # pos [B, S, 3] or [S, 3]
+    o = score_attention(q, k, v, softcap=50.0, causal=True, prefix=n_visual, q_doc=doc, k_doc=doc)
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from transfusion_amd import _lib as L
+from transfusion_amd import ops
+
+_POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _heads(name, t, like=None):
+    """A [B, S, H, D] operand with strides the kernels read as they are (channels contiguous, rows on 16 bytes), copied otherwise."""
+    ops._require_cuda(t)
+    if t.dim() != 4:
+        raise L.TfError(f"{name}: [batch, tokens, heads, head_dim] expected, got {tuple(t.shape)}")
+    ops._is_f32(t)
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise L.TfError(f"{name}: {t.dtype} on {t.device}, the queries are {like.dtype} on {like.device}")
+    return t
+
+
+def _rows(t):
+    """``t`` itself if its channels are contiguous and every row starts on 16 bytes, else a contiguous copy."""
+    e = t.element_size()
+    if t.numel() == 0:
+        return t
+    ok = (t.shape[3] == 1 or t.stride(3) == 1) and t.data_ptr() % 16 == 0
+    ok = ok and all(t.shape[i] == 1 or t.stride(i) * e % 16 == 0 for i in range(3))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t):
+    """Batch, token and head strides in elements; 0 for an axis of length 1 (torch leaves any number there)."""
+    return tuple(0 if t.shape[i] == 1 else t.stride(i) for i in range(3))
+
+
+def _ints(name, t, shape, dev):
+    """An int32 device tensor of exactly ``shape``, contiguous."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        raise L.TfError(f"{name}: an int32 tensor expected")
+    ops._require_cuda(t)
+    if t.device != dev or tuple(t.shape) != tuple(shape):
+        raise L.TfError(f"{name}: {tuple(t.shape)} on {t.device}, expected {tuple(shape)} on {dev}")
+    return t.contiguous()
+
+
+def _keep(dev, *tensors):
+    """Saved tensors may come from another stream's pool: the allocator must not hand their memory on before this stream has read it
+    (autograd drops them as soon as the backward is enqueued)."""
+    st = torch.cuda.current_stream(dev)
+    for t in tensors:
+        if t is not None and t.numel():
+            t.record_stream(st)
+
+
+# ------------------------------------------------------------------------------------------------------
+# rotary positions
+# ------------------------------------------------------------------------------------------------------
+class RotaryPlan:
+    """Which channel pair turns with which axis, and how fast: ``axes[a]`` pairs turn with axis ``a`` (in that order; a count of 0 leaves the
+    axis out).  Pair i of n on an axis has the frequency ``base ** (-i / n)``; with ``shared`` pair p of all P has ``base ** (-p / P)``
+    whatever its axis.  Pairs are the channels (p, P + p), or (2p, 2p + 1) with ``interleaved``; channels from 2 P on are not turned.
+    Holds two small device tensors; make it once a model, not once a call."""
+
+    def __init__(self, head_dim: int, axes, base: float = 10000.0, interleaved: bool = False, shared: bool = False, device="cuda"):
+        axes = tuple(int(n) for n in axes)
+        P = sum(axes)
+        if not axes or min(axes) < 0 or P == 0 or 2 * P > head_dim or P > 256:
+            raise L.TfError(f"RotaryPlan: {axes} channel pairs do not fit a head of {head_dim} channels (at most 256 pairs)")
+        if not (base > 0.0 and math.isfinite(base)):
+            raise L.TfError(f"RotaryPlan: base {base} must be positive and finite")
+        self.head_dim, self.axes, self.base, self.pairs = int(head_dim), axes, float(base), P
+        self.interleaved, self.shared = bool(interleaved), bool(shared)
+        if shared:
+            freq = [base ** (-p / P) for p in range(P)]
+        else:
+            freq = [base ** (-i / n) for n in axes for i in range(n)]
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise L.TfError("transfusion_amd kernels need device tensors on an MI355X (gfx950); there is no CPU fallback")
+        self.freq_rev = torch.tensor([f / (2.0 * math.pi) for f in freq], dtype=torch.float64).to(dev)
+        self.axis = torch.tensor([a for a, n in enumerate(axes) for _ in range(n)], dtype=torch.int32).to(dev)
+
+
+def _rotary_call(q, k, pos, plan, inverse):
+    dev = q.device
+    q, k = _rows(q), _rows(k) if k is not None else None
+    B, S, H, D = q.shape
+    qo = torch.empty(B, S, H, D, dtype=q.dtype, device=dev)
+    ko = None if k is None else torch.empty(B, S, k.shape[2], D, dtype=q.dtype, device=dev)
+    qs, ks = _strides(q), _strides(k) if k is not None else (0, 0, 0)
+    a = L.TfRotaryArgs(q=L.ptr(q), q_sb=qs[0], q_ss=qs[1], q_sh=qs[2], k=L.ptr(k), k_sb=ks[0], k_ss=ks[1], k_sh=ks[2], q_out=L.ptr(qo), k_out=L.ptr(ko),
+                       B=B, S=S, H=H, Hk=0 if k is None else k.shape[2], D=D, is_f32=ops._is_f32(q), pos=L.ptr(pos), pos_type=_POS_TYPES[pos.dtype],
+                       pos_batched=1 if pos.dim() == 3 else 0, n_axes=len(plan.axes), inv_freq=L.ptr(plan.freq_rev), axis=L.ptr(plan.axis),
+                       pairs=plan.pairs, interleaved=int(plan.interleaved), inverse=int(inverse))
+    with ops.on_device(dev):
+        L.call("tf_rotary", a, ops._stream())
+    return qo, ko
+
+
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, pos, plan):
+        ctx.save_for_backward(pos)
+        ctx.plan, ctx.shapes, ctx.dtype = plan, (q.shape, None if k is None else k.shape), q.dtype
+        if any(ctx.needs_input_grad[:2]):
+            _keep(q.device, pos)
+        ctx.set_materialize_grads(False)
+        qo, ko = _rotary_call(q, k, pos, plan, False)
+        return qo if k is None else (qo, ko)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        (pos,) = ctx.saved_tensors
+        live = [(i, g) for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[i]]
+        out = [None, None]
+        if live:
+            outs = _rotary_call(live[0][1], live[1][1] if len(live) > 1 else None, pos, ctx.plan, True)
+            for (i, _), g in zip(live, outs):
+                out[i] = g
+        return out[0], out[1], None, None
+
+
+def rotary(q, k, pos, plan: RotaryPlan):
+    """Turns the channel pairs of ``q`` [B, S, H, D] and ``k`` [B, S, Hk, D] (or None) by their tokens' positions -> new contiguous tensors
+    (a pair, or the turned ``q`` alone).  ``pos``: [B, S, len(axes)] or [S, len(axes)] int32, int64 or fp32 (fractional positions: a
+    coarse level's patches on a finer grid).  Positions take no gradient."""
+    _heads("rotary q", q)
+    if k is not None:
+        _heads("rotary k", k, like=q)
+        if k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+            raise L.TfError(f"rotary: k {tuple(k.shape)} does not match q {tuple(q.shape)}")
+    if not isinstance(plan, RotaryPlan) or plan.head_dim != q.shape[3] or plan.freq_rev.device != q.device:
+        raise L.TfError(f"rotary: a RotaryPlan of head_dim {q.shape[3]} on {q.device} expected")
+    ops._require_cuda(pos)
+    if pos.dtype not in _POS_TYPES or pos.device != q.device or pos.requires_grad:
+        raise L.TfError("rotary: positions are int32, int64 or fp32 tensors on the queries' device, without a gradient")
+    B, S = q.shape[:2]
+    if tuple(pos.shape) not in ((B, S, len(plan.axes)), (S, len(plan.axes))):
+        raise L.TfError(f"rotary: positions {tuple(pos.shape)}, expected {(B, S, len(plan.axes))} or {(S, len(plan.axes))}")
+    pos = pos.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        return _RotaryFn.apply(q, k, pos, plan)
+    qo, ko = _rotary_call(q, k, pos, plan, False)
+    return qo if k is None else (qo, ko)
+
+
+# ------------------------------------------------------------------------------------------------------
+# attention with changed scores
+# ------------------------------------------------------------------------------------------------------
+def _score_args(q, k, v, out, opt):
+    scale, softcap, slopes, causal, prefix, q_start, q_doc, k_doc = opt
+    B, Sq, H, D = q.shape
+    qs, ks, vs = _strides(q), _strides(k), _strides(v)
+    return L.TfScoreAttnArgs(q=L.ptr(q), q_sb=qs[0], q_ss=qs[1], q_sh=qs[2], k=L.ptr(k), k_sb=ks[0], k_ss=ks[1], k_sh=ks[2],
+                             v=L.ptr(v), v_sb=vs[0], v_ss=vs[1], v_sh=vs[2], out=L.ptr(out), B=B, Sq=Sq, Sk=k.shape[1], H=H, Hk=k.shape[2], D=D,
+                             is_f32=ops._is_f32(q), scale=scale, softcap=softcap, slopes=L.ptr(slopes), causal=causal, prefix=L.ptr(prefix),
+                             q_start=L.ptr(q_start), q_doc=L.ptr(q_doc), k_doc=L.ptr(k_doc))
+
+
+def _score_fwd(q, k, v, opt, want_lse):
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    B, Sq, H, D = q.shape
+    out = torch.empty(B, Sq, H, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, Sq, dtype=torch.float32, device=q.device) if want_lse else None
+    a = _score_args(q, k, v, out, opt)
+    a.lse = L.ptr(lse)
+    need = L.load().tf_score_attn_work(L.C.byref(a))
+    if need:
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.work, a.work_bytes = L.ptr(work), need
+    with ops.on_device(q.device):
+        L.call("tf_score_attn_fwd", a, ops._stream())
+    return q, k, v, out, lse
+
+
+class _ScoreAttnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, scale, softcap, causal, prefix, q_start, q_doc, k_doc):
+        opt = (scale, softcap, slopes, causal, prefix, q_start, q_doc, k_doc)
+        q, k, v, out, lse = _score_fwd(q, k, v, opt, True)
+        _keep(q.device, q, k, v, slopes, prefix, q_start, q_doc, k_doc)
+        ctx.save_for_backward(q, k, v, slopes, out, lse, prefix, q_start, q_doc, k_doc)
+        ctx.opt = (scale, softcap, causal)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go):
+        q, k, v, slopes, out, lse, prefix, q_start, q_doc, k_doc = ctx.saved_tensors
+        scale, softcap, causal = ctx.opt
+        dev = q.device
+        go = _rows(go)
+        a = _score_args(q, k, v, out, (scale, softcap, slopes, causal, prefix, q_start, q_doc, k_doc))
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
+        delta = torch.empty_like(lse)
+        a.lse, a.delta, a.dq, a.dk, a.dv, a.dout = L.ptr(lse), L.ptr(delta), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.ptr(go)
+        a.do_sb, a.do_ss, a.do_sh = _strides(go)
+        ds = None
+        if slopes is not None and ctx.needs_input_grad[3]:
+            ds, rows = torch.empty_like(slopes), torch.empty_like(lse)
+            a.dslopes, a.dslope_rows = L.ptr(ds), L.ptr(rows)
+        with ops.on_device(dev):
+            L.call("tf_score_attn_bwd", a, ops._stream())
+        return dq, dk, dv, ds, None, None, None, None, None, None, None
+
+
+def score_attention(q, k, v, scale: float = None, softcap: float = 0.0, slopes=None, causal: bool = False, prefix=None, q_start=None,
+                    q_doc=None, k_doc=None):
+    """softmax(change(scale q k^T)) v -> [B, Sq, H, D], differentiable in ``q`` [B, Sq, H, D], ``k`` / ``v`` [B, Sk, Hk, D] (H a multiple of
+    Hk: consecutive heads share) and ``slopes``.  A query at position p = ``q_start[b]`` + i (default: the queries are the last Sq of the
+    Sk tokens) sees key j with the score
+
+        s = scale q.k;   softcap tanh(s / softcap) if softcap > 0;   - slopes[h] |p - j|   (slopes: fp32 [H])
+
+    unless it is hidden: ``causal`` hides j > p except the first ``prefix[b]`` keys (int32 [B]); ``q_doc`` / ``k_doc`` (int32 [B, Sq] /
+    [B, Sk]) hide keys of other documents, and a negative document is padding: attends nothing, is attended by nobody, and whatever its
+    rows hold is not used.  A query that sees nothing gets zeros.  ``scale`` defaults to 1 / sqrt(D).  D <= 256, a multiple of 8."""
+    _heads("score_attention q", q)
+    _heads("score_attention k", k, like=q)
+    _heads("score_attention v", v, like=q)
+    B, Sq, H, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise L.TfError(f"score_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not belong together")
+    if H == 0 or Hk == 0 or H % Hk:
+        raise L.TfError(f"score_attention: {H} query heads cannot share {Hk} key heads")
+    if D == 0 or D > 256 or D % 8:
+        raise L.TfError(f"score_attention: head_dim {D} must be a multiple of 8, at most 256")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    softcap = float(softcap)
+    if not math.isfinite(scale) or not (0.0 <= softcap < math.inf):
+        raise L.TfError(f"score_attention: scale {scale} must be finite, softcap {softcap} finite and not negative")
+    dev = q.device
+    if slopes is not None:
+        ops._require_cuda(slopes)
+        if slopes.dtype != torch.float32 or tuple(slopes.shape) != (H,) or slopes.device != dev:
+            raise L.TfError(f"score_attention: slopes must be fp32 [{H}] on {dev}")
+        slopes = slopes.contiguous()
+    if prefix is not None:
+        if not causal:
+            raise L.TfError("score_attention: a prefix needs causal=True (without it every key is visible)")
+        prefix = _ints("score_attention prefix", prefix, (B,), dev)
+    if q_start is not None:
+        q_start = _ints("score_attention q_start", q_start, (B,), dev)
+    if (q_doc is None) != (k_doc is None):
+        raise L.TfError("score_attention: q_doc and k_doc come together")
+    if q_doc is not None:
+        q_doc = _ints("score_attention q_doc", q_doc, (B, Sq), dev)
+        k_doc = _ints("score_attention k_doc", k_doc, (B, Sk), dev)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, slopes)):
+        return _ScoreAttnFn.apply(q, k, v, slopes, scale, softcap, int(bool(causal)), prefix, q_start, q_doc, k_doc)
+    return _score_fwd(q, k, v, (scale, softcap, slopes, int(bool(causal)), prefix, q_start, q_doc, k_doc), False)[3]

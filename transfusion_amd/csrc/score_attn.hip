@@ -1,0 +1,655 @@
+// Attention whose scores are changed before the softmax: capped by a tanh, biased by distance, masked by documents and by a causal
+// horizon with a bidirectional prefix.  For query i at position p and key j of one head
+//   s = scale * q.k ;  s = cap * tanh(s / cap) (cap > 0) ;  s -= slope_h * |p - j| ;
+//   hidden unless  doc_q == doc_k >= 0  and  (not causal or j <= p or j < prefix) ;   P = softmax_j(s) ;  o = P v .
+// A row that attends nothing gives o = 0 and no gradient.  Heads may share keys and values (H / Hk heads each).
+//
+// No [Sq, Sk] tensor reaches memory: the forward keeps a running maximum and sum and stores one log-sum-exp a row, the backward forms P
+// again from it.  Orientation as in attn_bf16.hip: the score tile is computed transposed (keys in the accumulator registers, the query
+// on the lane), so a row's statistics are one scalar a lane and the tile is the next product's operand as it stands.
+//   score_fwd_kernel   query on the lane, loops over key tiles                       -> o, lse
+//   score_dq_kernel    query on the lane, loops over key tiles                       -> dq, delta = rowsum(dO o), the slopes' row sums
+//   score_dkv_kernel   key on the lane, loops over the heads of its group and their query tiles -> dk, dv (no atomics)
+// Scores, statistics and accumulators are fp32.  P and dS are rounded to the operand type of the next product (bf16: half a step, 2^-9
+// of each term); fp32 tensors run on the fp32 matrix instructions throughout.
+#include "tf_common.h"
+#include "tf_kernels.h"
+#include "attn_common.h"
+#include <atomic>
+
+namespace {
+
+// ---- operand fragments: 8 consecutive channels of one row per lane (half h of the wave holds channels 16 ks + 8 h ..) ----
+template <bool F32> struct SFrag;
+template <> struct SFrag<false> { u32x4 v; };
+template <> struct SFrag<true> { f32x4 a, b; };
+
+template <bool F32> __device__ __forceinline__ f32x16 smma(const SFrag<F32>& A, const SFrag<F32>& B, f32x16 c) {
+  if constexpr (F32) {
+    // step e multiplies channel e of both halves: the k order inside the 16 channels is the same for both operands, so any will do
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(A.a[e], B.a[e], c, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(A.b[e], B.b[e], c, 0, 0, 0);
+    return c;
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(A.v), as_bf16x8(B.v), c, 0, 0, 0);
+  }
+}
+
+template <bool F32, int HDP> struct STile {
+  static constexpr int ESZ = F32 ? 4 : 2;
+  static constexpr int STR = F32 ? HDP * 4 + 16 : Geo<HDP>::TSTR;       // fp32: rows 4 banks apart
+  static constexpr int CPR = HDP * ESZ / 16;                            // 16-byte pieces of a row
+  static __device__ __forceinline__ int off(int row, int c) {
+    if constexpr (F32) return row * STR + c * 16;
+    else return tile_off(row, c, STR);
+  }
+  // rows row0 .. row0 + ROWS - 1 of a [*, row_bytes] matrix into LDS; rows at or beyond row_end, rows whose document is negative and
+  // channels at or beyond D arrive as zeros, whatever memory holds there
+  template <int ROWS> static __device__ __forceinline__ void stage(unsigned char* lds, const char* base, long long row_bytes, int row0, int row_end,
+                                                                   const int* doc, int D, int tid) {
+    for (int id = tid; id < ROWS * CPR; id += 256) {
+      const int r = id / CPR, c = id % CPR, gr = row0 + r;
+      u32x4 v = {0, 0, 0, 0};
+      if (gr < row_end && c * (16 / ESZ) < D && (doc == nullptr || doc[gr] >= 0)) v = *(const u32x4*)(base + (long long)gr * row_bytes + c * 16);
+      *(u32x4*)(lds + off(r, c)) = v;
+    }
+  }
+  static __device__ __forceinline__ SFrag<F32> row(const unsigned char* tile, int row0, int ks, int lane) {
+    SFrag<F32> f;
+    if constexpr (F32) {
+      const unsigned char* p = tile + (row0 + (lane & 31)) * STR + (ks * 16 + 8 * (lane >> 5)) * 4;
+      f.a = *(const f32x4*)p;
+      f.b = *(const f32x4*)(p + 16);
+    } else {
+      f.v = *(const u32x4*)(tile + tile_off(row0 + (lane & 31), 2 * ks + (lane >> 5), STR));
+    }
+    return f;
+  }
+  // c[channel col0 + ..][lane's row] += sum over 32 tile rows (krow0 ..) of tile[row][channel] * p[row]: p is an accumulator tile
+  static __device__ __forceinline__ f32x16 mma_t(const unsigned char* tile, int krow0, int col0, const f32x16& p, f32x16 c, int lane) {
+    if constexpr (F32) {
+      const float* t = (const float*)(tile + (krow0 + 4 * (lane >> 5)) * STR) + col0 + (lane & 31);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) c = __builtin_amdgcn_mfma_f32_32x32x2f32(t[((r & 3) + 8 * (r >> 2)) * (STR / 4)], p[r], c, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tr_frag<HDP>(tile, krow0 + 16 * s, col0, lane), acc_frag(p, s), c, 0, 0, 0);
+    }
+    return c;
+  }
+};
+
+// fragment of one row straight from memory; `ok` false: zeros
+template <bool F32> __device__ __forceinline__ SFrag<F32> gfrag(const char* row, int ks, int h, int D, bool ok) {
+  SFrag<F32> f;
+  const int c0 = ks * 16 + 8 * h;
+  ok = ok && c0 < D;
+  if constexpr (F32) {
+    f.a = ok ? *(const f32x4*)(row + c0 * 4) : f32x4{0, 0, 0, 0};
+    f.b = ok ? *(const f32x4*)(row + c0 * 4 + 16) : f32x4{0, 0, 0, 0};
+  } else {
+    f.v = ok ? *(const u32x4*)(row + c0 * 2) : u32x4{0, 0, 0, 0};
+  }
+  return f;
+}
+template <bool F32> __device__ __forceinline__ float frag_dot(const SFrag<F32>& x, const SFrag<F32>& y) {
+  float s = 0.f;
+  if constexpr (F32) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s += x.a[e] * y.a[e] + x.b[e] * y.b[e];
+  } else {
+    float a[8], b[8];
+    unpack8(x.v, a);
+    unpack8(y.v, b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += a[e] * b[e];
+  }
+  return s;
+}
+
+// ---- the change of a score, in the log2 domain ----
+struct SMod {
+  float sc;          // no cap: scale * log2 e;  cap: 2 log2 e * scale / cap (the exponent of the tanh)
+  float capl;        // cap * log2 e, or 0
+  float slope2;      // slope * log2 e
+};
+template <bool F32> __device__ __forceinline__ float tanh_of(float y2) {       // y2 = 2 log2(e) y
+  if constexpr (F32) return tanhf(y2 * 0.34657359027997264f);
+  // 1 - 2 / (1 + e^2y): absolute error ~1e-7 (the bf16 product's own error is larger); +-inf give +-1, no NaN in between
+  return 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + fast_exp2(y2));
+}
+__device__ __forceinline__ SMod smod(const TfScoreAttnArgs& a, int head) {
+  SMod m;
+  m.capl = a.softcap > 0.f ? a.softcap * LOG2E : 0.f;
+  m.sc = a.softcap > 0.f ? 2.f * LOG2E * a.scale / a.softcap : a.scale * LOG2E;
+  m.slope2 = a.slopes != nullptr ? a.slopes[head] * LOG2E : 0.f;
+  return m;
+}
+// position of query 0 (bounded so that sums with a query number stay in 32 bits) and the prefix length of sample b
+__device__ __forceinline__ int q_pos0(const TfScoreAttnArgs& a, int b) {
+  const int p = a.q_start != nullptr ? a.q_start[b] : a.Sk - a.Sq;
+  return min(max(p, -(1 << 30)), 1 << 30);
+}
+__device__ __forceinline__ int prefix_of(const TfScoreAttnArgs& a, int b) { return a.prefix != nullptr ? min(max(a.prefix[b], 0), a.Sk) : 0; }
+
+constexpr float S_NEG = -1.0e38f;          // the running maximum before the first visible key
+
+// ================================================================================================
+// forward
+// ================================================================================================
+template <bool F32, int HDP>
+__global__ __launch_bounds__(256, 1) void score_fwd_kernel(const TfScoreAttnArgs a, int nqb, int nsplit, int split_tiles) {
+  using T = STile<F32, HDP>;
+  constexpr int KT = F32 ? 32 : 64, NKB = KT / 32, KS = HDP / 16, DB = HDP / 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* kt = smem;
+  unsigned char* vt = smem + KT * T::STR;
+  int* docs = (int*)(smem + 2 * KT * T::STR);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  const int logical = xcd_remap(blockIdx.x, gridDim.x);
+  const int split = logical % nsplit, t1 = logical / nsplit;
+  const int qb = nqb - 1 - t1 % nqb, bh = t1 / nqb, b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.Hk);
+  const char* qbase = (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * T::ESZ;
+  const char* kbase = (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * T::ESZ;
+  const char* vbase = (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * T::ESZ;
+  const int* kdoc = a.k_doc != nullptr ? a.k_doc + (size_t)b * a.Sk : nullptr;
+  const SMod m = smod(a, head);
+  const int p0 = q_pos0(a, b), pfx = prefix_of(a, b);
+  const int i = qb * 128 + wave * 32 + (lane & 31);
+  const int qd = kdoc != nullptr && i < a.Sq ? a.q_doc[(size_t)b * a.Sq + i] : 0;
+  const bool live = i < a.Sq && qd >= 0;
+  const int p = p0 + i;
+  const int lim = !live ? -1 : (a.causal ? min(max(p, pfx - 1), a.Sk - 1) : a.Sk - 1);       // last key this row may see
+  const int i_last = min(qb * 128 + 127, a.Sq - 1);
+  const int hi = a.causal ? min(max(p0 + i_last + 1, pfx), a.Sk) : a.Sk;                      // one past the block's last
+  const int tile_end = (max(hi, 0) + KT - 1) / KT;
+  const int t_lo = split * split_tiles, t_hi = min(tile_end, t_lo + split_tiles);
+  SFrag<F32> qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) qf[ks] = gfrag<F32>(qbase + (long long)min(i, a.Sq - 1) * a.q_ss * T::ESZ, ks, h, a.D, live);
+  f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m_run = S_NEG, l_run = 0.f;
+  for (int t = t_lo; t < t_hi; ++t) {
+    const int kv0 = t * KT;
+    __syncthreads();
+    T::template stage<KT>(kt, kbase, a.k_ss * T::ESZ, kv0, hi, kdoc, a.D, tid);
+    T::template stage<KT>(vt, vbase, a.v_ss * T::ESZ, kv0, hi, kdoc, a.D, tid);
+    if (kdoc != nullptr && tid < KT) docs[tid] = kv0 + tid < a.Sk ? kdoc[kv0 + tid] : -1;
+    __syncthreads();
+    f32x16 st[NKB];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[kb][r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) st[kb] = smma<F32>(T::row(kt, kb * 32, ks, lane), qf[ks], st[kb]);
+    }
+    const float pd = (float)(p - kv0 - 4 * h);
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int j = kb * 32 + (r & 3) + 8 * (r >> 2);
+        float x = m.capl != 0.f ? m.capl * tanh_of<F32>(st[kb][r] * m.sc) : st[kb][r] * m.sc;
+        if (m.slope2 != 0.f) x -= m.slope2 * fabsf(pd - (float)j);
+        bool vis = kv0 + j + 4 * h <= lim;
+        if (kdoc != nullptr) vis = vis && docs[j + 4 * h] == qd;
+        st[kb][r] = vis ? x : -INFINITY;
+      }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[kb][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float m_new = fmaxf(m_run, mx), alpha = fast_exp2(m_run - m_new);
+    m_run = m_new;
+    l_run *= alpha;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        st[kb][r] = fast_exp2(st[kb][r] - m_run);
+        l_run += st[kb][r];
+      }
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb) o[d] = T::mma_t(vt, kb * 32, d * 32, st[kb], o[d], lane);
+  }
+  const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+  if (i >= a.Sq) return;
+  const long long rows = (long long)a.B * a.H * a.Sq, row = (long long)bh * a.Sq + i;
+  if (nsplit > 1) {                       // unnormalised part of this range of keys; score_join_kernel adds them up
+    float* po = (float*)a.work + ((long long)split * rows + row) * a.D;
+    float* pml = (float*)a.work + (long long)nsplit * rows * a.D + ((long long)split * rows + row) * 2;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = d * 32 + 8 * g + 4 * h;
+        if (c < a.D) *(f32x4*)(po + c) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+      }
+    if (h == 0) { pml[0] = m_run; pml[1] = l_tot; }
+    return;
+  }
+  const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;
+  char* orow = (char*)a.out + (((long long)b * a.Sq + i) * a.H + head) * a.D * T::ESZ;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = d * 32 + 8 * g + 4 * h;
+      if (c >= a.D) continue;
+      const float x0 = o[d][4 * g] * inv, x1 = o[d][4 * g + 1] * inv, x2 = o[d][4 * g + 2] * inv, x3 = o[d][4 * g + 3] * inv;
+      if constexpr (F32) *(f32x4*)(orow + c * 4) = f32x4{x0, x1, x2, x3};
+      else *(u32x2*)(orow + c * 2) = u32x2{pack2bf(x0, x1), pack2bf(x2, x3)};
+    }
+  // rows without keys: +inf, so that every probability formed from it again is 0
+  if (h == 0 && a.lse != nullptr) a.lse[row] = l_tot == 0.f ? INFINITY : m_run + log2f(l_tot);
+}
+
+// joins the parts of a split forward: one wave a row, four channels a lane
+template <bool F32> __global__ __launch_bounds__(256) void score_join_kernel(const TfScoreAttnArgs a, int nsplit) {
+  const long long rows = (long long)a.B * a.H * a.Sq, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  const float* po = (const float*)a.work + row * a.D;
+  const float* pml = (const float*)a.work + (long long)nsplit * rows * a.D + row * 2;
+  float mx = S_NEG;
+  for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, pml[(long long)s * rows * 2]);
+  float l = 0.f;
+  f32x4 acc = {0, 0, 0, 0};
+  for (int s = 0; s < nsplit; ++s) {
+    const float w = fast_exp2(pml[(long long)s * rows * 2] - mx);
+    l += w * pml[(long long)s * rows * 2 + 1];
+    if (lane * 4 < a.D) acc += w * *(const f32x4*)(po + (long long)s * rows * a.D + lane * 4);
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const int i = (int)(row % a.Sq), bh = (int)(row / a.Sq), b = bh / a.H, head = bh % a.H;
+  const long long oo = (((long long)b * a.Sq + i) * a.H + head) * a.D + lane * 4;
+  if (lane * 4 < a.D) {
+    if constexpr (F32) *(f32x4*)((float*)a.out + oo) = acc * inv;
+    else *(u32x2*)((u16*)a.out + oo) = u32x2{pack2bf(acc[0] * inv, acc[1] * inv), pack2bf(acc[2] * inv, acc[3] * inv)};
+  }
+  if (lane == 0 && a.lse != nullptr) a.lse[row] = l == 0.f ? INFINITY : mx + log2f(l);
+}
+
+// ================================================================================================
+// backward: dq
+// ================================================================================================
+template <bool F32, int HDP>
+__global__ __launch_bounds__(256, 1) void score_dq_kernel(const TfScoreAttnArgs a, int nqb) {
+  using T = STile<F32, HDP>;
+  constexpr int KT = 32, KS = HDP / 16, DB = HDP / 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* kt = smem;
+  unsigned char* vt = smem + KT * T::STR;
+  int* docs = (int*)(smem + 2 * KT * T::STR);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  const int logical = xcd_remap(blockIdx.x, gridDim.x);
+  const int qb = nqb - 1 - logical % nqb, bh = logical / nqb, b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.Hk);
+  const char* qbase = (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * T::ESZ;
+  const char* kbase = (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * T::ESZ;
+  const char* vbase = (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * T::ESZ;
+  const int* kdoc = a.k_doc != nullptr ? a.k_doc + (size_t)b * a.Sk : nullptr;
+  const SMod m = smod(a, head);
+  const int p0 = q_pos0(a, b), pfx = prefix_of(a, b);
+  const int i = qb * 128 + wave * 32 + (lane & 31), ic = min(i, a.Sq - 1);
+  const int qd = kdoc != nullptr && i < a.Sq ? a.q_doc[(size_t)b * a.Sq + i] : 0;
+  const bool live = i < a.Sq && qd >= 0;
+  const int p = p0 + i;
+  const int lim = !live ? -1 : (a.causal ? min(max(p, pfx - 1), a.Sk - 1) : a.Sk - 1);
+  const int i_last = min(qb * 128 + 127, a.Sq - 1);
+  const int hi = a.causal ? min(max(p0 + i_last + 1, pfx), a.Sk) : a.Sk;
+  const int tile_end = (max(hi, 0) + KT - 1) / KT;
+  const long long row = (long long)bh * a.Sq + ic;
+  // fp32 heads of 256: Q, dO and dq together do not fit the register file, Q is read again (from L1 / L2) for every tile
+  constexpr bool REREAD = F32 && HDP > 192;
+  const char* qrow = qbase + (long long)ic * a.q_ss * T::ESZ;
+  SFrag<F32> qf[REREAD ? 1 : KS], dof[KS];
+  float delta = 0.f;
+  {
+    const char* orow = (const char*)a.out + (((long long)b * a.Sq + ic) * a.H + head) * a.D * T::ESZ;
+    const char* drow = (const char*)a.dout + ((long long)b * a.do_sb + (long long)ic * a.do_ss + (long long)head * a.do_sh) * T::ESZ;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if constexpr (!REREAD) qf[ks] = gfrag<F32>(qrow, ks, h, a.D, live);
+      dof[ks] = gfrag<F32>(drow, ks, h, a.D, live);
+      delta += frag_dot<F32>(dof[ks], gfrag<F32>(orow, ks, h, a.D, live));
+    }
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  const float lse = live ? a.lse[row] : INFINITY;
+  f32x16 dq[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
+  float dsl = 0.f;
+  for (int t = 0; t < tile_end; ++t) {
+    const int kv0 = t * KT;
+    __syncthreads();
+    T::template stage<KT>(kt, kbase, a.k_ss * T::ESZ, kv0, hi, kdoc, a.D, tid);
+    T::template stage<KT>(vt, vbase, a.v_ss * T::ESZ, kv0, hi, kdoc, a.D, tid);
+    if (kdoc != nullptr && tid < KT) docs[tid] = kv0 + tid < a.Sk ? kdoc[kv0 + tid] : -1;
+    __syncthreads();
+    f32x16 st, dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if constexpr (REREAD) st = smma<F32>(T::row(kt, 0, ks, lane), gfrag<F32>(qrow, ks, h, a.D, live), st);
+      else st = smma<F32>(T::row(kt, 0, ks, lane), qf[ks], st);
+      dp = smma<F32>(T::row(vt, 0, ks, lane), dof[ks], dp);
+    }
+    const float pd = (float)(p - kv0 - 4 * h);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int j = (r & 3) + 8 * (r >> 2);
+      const float th = m.capl != 0.f ? tanh_of<F32>(st[r] * m.sc) : 0.f, dist = fabsf(pd - (float)j);
+      float x = m.capl != 0.f ? m.capl * th : st[r] * m.sc;
+      if (m.slope2 != 0.f) x -= m.slope2 * dist;
+      bool vis = kv0 + j + 4 * h <= lim;
+      if (kdoc != nullptr) vis = vis && docs[j + 4 * h] == qd;
+      const float ds = vis ? fast_exp2(x - lse) * (dp[r] - delta) : 0.f;
+      dsl -= ds * dist;
+      st[r] = ds * (1.f - th * th);
+    }
+#pragma unroll
+    for (int d = 0; d < DB; ++d) dq[d] = T::mma_t(kt, 0, d * 32, st, dq[d], lane);
+  }
+  dsl += __shfl_xor(dsl, 32, 64);
+  if (i >= a.Sq) return;
+  if (h == 0) {
+    a.delta[row] = delta;
+    if (a.dslopes != nullptr) a.dslope_rows[row] = dsl;
+  }
+  char* grow = (char*)a.dq + (((long long)b * a.Sq + i) * a.H + head) * a.D * T::ESZ;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = d * 32 + 8 * g + 4 * h;
+      if (c >= a.D) continue;
+      const float x0 = dq[d][4 * g] * a.scale, x1 = dq[d][4 * g + 1] * a.scale, x2 = dq[d][4 * g + 2] * a.scale, x3 = dq[d][4 * g + 3] * a.scale;
+      if constexpr (F32) *(f32x4*)(grow + c * 4) = f32x4{x0, x1, x2, x3};
+      else *(u32x2*)(grow + c * 2) = u32x2{pack2bf(x0, x1), pack2bf(x2, x3)};
+    }
+}
+
+// the slopes' gradient: one workgroup a head adds the rows of all samples up, in 64 bits and in one order
+__global__ __launch_bounds__(256) void score_dslope_kernel(const float* __restrict__ rows, float* __restrict__ out, int B, int H, int Sq) {
+  __shared__ double sh[256];
+  const int head = blockIdx.x, tid = threadIdx.x;
+  double s = 0.0;
+  for (int b = 0; b < B; ++b) {
+    const float* r = rows + ((size_t)b * H + head) * Sq;
+    for (int i = tid; i < Sq; i += 256) s += (double)r[i];
+  }
+  sh[tid] = s;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (tid < o) sh[tid] += sh[tid + o];
+    __syncthreads();
+  }
+  if (tid == 0) out[head] = (float)sh[0];
+}
+
+// ================================================================================================
+// backward: dk, dv.  PART 0: dv, 1: dk, 2: both (wide heads do not hold both accumulators beside the operands)
+// ================================================================================================
+template <bool F32, int HDP, int PART>
+__global__ __launch_bounds__(256, 1) void score_dkv_kernel(const TfScoreAttnArgs a, int nkb) {
+  using T = STile<F32, HDP>;
+  constexpr int QT = 32, KS = HDP / 16, DB = HDP / 32;
+  constexpr bool DK = PART != 0, DV = PART != 1;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* qt = smem;
+  unsigned char* dot = smem + QT * T::STR;
+  float* lse_s = (float*)(smem + 2 * QT * T::STR);
+  float* del_s = lse_s + QT;
+  int* lim_s = (int*)(del_s + QT);
+  int* doc_s = lim_s + QT;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  const int logical = xcd_remap(blockIdx.x, gridDim.x);
+  const int kb = logical % nkb, bk = logical / nkb, b = bk / a.Hk, kvh = bk % a.Hk, G = a.H / a.Hk;
+  const char* kbase = (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * T::ESZ;
+  const char* vbase = (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * T::ESZ;
+  const int* kdoc = a.k_doc != nullptr ? a.k_doc + (size_t)b * a.Sk : nullptr;
+  const int* qdoc = a.k_doc != nullptr ? a.q_doc + (size_t)b * a.Sq : nullptr;
+  const int p0 = q_pos0(a, b), pfx = prefix_of(a, b);
+  const int k0 = kb * 128, j = k0 + wave * 32 + (lane & 31), jc = min(j, a.Sk - 1);
+  const int kd = kdoc != nullptr ? (j < a.Sk ? kdoc[j] : -1) : 0;
+  const bool live = j < a.Sk && kd >= 0;
+  constexpr bool REREAD = F32 && HDP > 192;                   // as in score_dq_kernel: V is read again for every tile
+  const char* vrow = vbase + (long long)jc * a.v_ss * T::ESZ;
+  SFrag<F32> kf[KS], vf[DK && !REREAD ? KS : 1];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    kf[ks] = gfrag<F32>(kbase + (long long)jc * a.k_ss * T::ESZ, ks, h, a.D, live);
+    if constexpr (DK && !REREAD) vf[ks] = gfrag<F32>(vrow, ks, h, a.D, live);
+  }
+  f32x16 dk[DK ? DB : 1], dv[DV ? DB : 1];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if (DK) dk[d][r] = 0.f;
+      if (DV) dv[d][r] = 0.f;
+    }
+  // the first query that may see a key of this block
+  const int i_lo = a.causal && k0 >= pfx ? min(max(k0 - p0, 0), a.Sq) : 0;
+  for (int g = 0; g < G; ++g) {
+    const int head = kvh * G + g;
+    const SMod m = smod(a, head);
+    const char* qbase = (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * T::ESZ;
+    const char* dbase = (const char*)a.dout + ((long long)b * a.do_sb + (long long)head * a.do_sh) * T::ESZ;
+    const long long row0 = ((long long)b * a.H + head) * a.Sq;
+    for (int i0 = i_lo / QT * QT; i0 < a.Sq; i0 += QT) {
+      __syncthreads();
+      T::template stage<QT>(qt, qbase, a.q_ss * T::ESZ, i0, a.Sq, qdoc, a.D, tid);
+      T::template stage<QT>(dot, dbase, a.do_ss * T::ESZ, i0, a.Sq, qdoc, a.D, tid);
+      if (tid < QT) {
+        const int i = i0 + tid, p = p0 + i, qd = qdoc != nullptr && i < a.Sq ? qdoc[i] : 0;
+        const bool ok = i < a.Sq && qd >= 0;
+        lse_s[tid] = ok ? a.lse[row0 + i] : INFINITY;
+        del_s[tid] = ok ? a.delta[row0 + i] : 0.f;
+        lim_s[tid] = !ok ? -1 : (a.causal ? max(p, pfx - 1) : a.Sk - 1);
+        doc_s[tid] = qd;
+      }
+      __syncthreads();
+      f32x16 st, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        st = smma<F32>(T::row(qt, 0, ks, lane), kf[ks], st);
+        if constexpr (DK && REREAD) dp = smma<F32>(T::row(dot, 0, ks, lane), gfrag<F32>(vrow, ks, h, a.D, live), dp);
+        else if constexpr (DK) dp = smma<F32>(T::row(dot, 0, ks, lane), vf[ks], dp);
+      }
+      const float pd = (float)(p0 + i0 + 4 * h - j);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int q = (r & 3) + 8 * (r >> 2), qq = q + 4 * h;
+        const float th = m.capl != 0.f ? tanh_of<F32>(st[r] * m.sc) : 0.f;
+        float x = m.capl != 0.f ? m.capl * th : st[r] * m.sc;
+        if (m.slope2 != 0.f) x -= m.slope2 * fabsf(pd + (float)q);
+        const bool vis = live && j <= lim_s[qq] && doc_s[qq] == kd;
+        const float pr = vis ? fast_exp2(x - lse_s[qq]) : 0.f;
+        if (DK) dp[r] = vis ? pr * (dp[r] - del_s[qq]) * (1.f - th * th) : 0.f;
+        st[r] = pr;
+      }
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        if (DV) dv[d] = T::mma_t(dot, 0, d * 32, st, dv[d], lane);
+        if (DK) dk[d] = T::mma_t(qt, 0, d * 32, dp, dk[d], lane);
+      }
+    }
+  }
+  if (j >= a.Sk) return;
+  const long long go = (((long long)b * a.Sk + j) * a.Hk + kvh) * a.D;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = d * 32 + 8 * g + 4 * h;
+      if (c >= a.D) continue;
+      if (DK) {
+        const float x0 = dk[d][4 * g] * a.scale, x1 = dk[d][4 * g + 1] * a.scale, x2 = dk[d][4 * g + 2] * a.scale, x3 = dk[d][4 * g + 3] * a.scale;
+        if constexpr (F32) *(f32x4*)((float*)a.dk + go + c) = f32x4{x0, x1, x2, x3};
+        else *(u32x2*)((u16*)a.dk + go + c) = u32x2{pack2bf(x0, x1), pack2bf(x2, x3)};
+      }
+      if (DV) {
+        const float x0 = dv[d][4 * g], x1 = dv[d][4 * g + 1], x2 = dv[d][4 * g + 2], x3 = dv[d][4 * g + 3];
+        if constexpr (F32) *(f32x4*)((float*)a.dv + go + c) = f32x4{x0, x1, x2, x3};
+        else *(u32x2*)((u16*)a.dv + go + c) = u32x2{pack2bf(x0, x1), pack2bf(x2, x3)};
+      }
+    }
+}
+
+// ================================================================================================
+// launchers
+// ================================================================================================
+// dynamic LDS beyond the default limit is granted per device
+template <class K> void allow_lds(K kern, size_t bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev > 63) dev = 0;
+  if (done.load(std::memory_order_relaxed) >> dev & 1ull) return;
+  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  done.fetch_or(1ull << dev, std::memory_order_relaxed);
+}
+
+int hdp_of(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : D <= 192 ? 192 : 256; }
+
+struct FwdPlan { int nqb, nsplit, split_tiles; };
+FwdPlan fwd_plan(const TfScoreAttnArgs* a) {
+  FwdPlan f;
+  const int kt = a->is_f32 ? 32 : 64;
+  f.nqb = (a->Sq + 127) / 128;
+  const long long blocks = (long long)a->B * a->H * f.nqb;
+  const int tiles = std::max(1, (a->Sk + kt - 1) / kt);
+  long long want = blocks >= 256 ? 1 : std::min<long long>((512 + blocks - 1) / blocks, tiles / 4);
+  if (want < 1) want = 1;
+  f.split_tiles = (int)((tiles + want - 1) / want);
+  f.nsplit = (tiles + f.split_tiles - 1) / f.split_tiles;
+  return f;
+}
+
+int check(const TfScoreAttnArgs* a) {
+  if (a->B < 0 || a->Sq < 0 || a->Sk < 0 || a->H <= 0 || a->Hk <= 0 || a->H % a->Hk != 0) return -1;
+  if (a->D <= 0 || a->D > 256 || a->D % 8 != 0) return -2;
+  if (!(a->softcap >= 0.f)) return -3;
+  if ((a->k_doc == nullptr) != (a->q_doc == nullptr) && a->Sq > 0 && a->Sk > 0) return -4;
+  const long long blocks = (long long)a->B * std::max(a->H * ((a->Sq + 127ll) / 128), (long long)a->Hk * ((a->Sk + 127) / 128));
+  if (blocks > 0x3fffff || (long long)a->Sq + a->Sk > (1ll << 30)) return -5;
+  return 0;
+}
+bool aligned(const void* p, long long sb, long long ss, long long sh, int e) {
+  return (((uintptr_t)p) & 15) == 0 && sb * e % 16 == 0 && ss * e % 16 == 0 && sh * e % 16 == 0;
+}
+
+template <bool F32, int HDP> int launch_fwd(const TfScoreAttnArgs* a, hipStream_t st) {
+  constexpr int KT = F32 ? 32 : 64;
+  const FwdPlan f = fwd_plan(a);
+  const size_t lds = 2 * KT * STile<F32, HDP>::STR + KT * 4;
+  allow_lds(score_fwd_kernel<F32, HDP>, lds);
+  {
+    TfTraceScope tr(F32 ? "score_fwd_kernel<fp32>" : "score_fwd_kernel<bf16>", st, 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D);
+    hipLaunchKernelGGL((score_fwd_kernel<F32, HDP>), dim3(a->B * a->H * f.nqb * f.nsplit), dim3(256), lds, st, *a, f.nqb, f.nsplit, f.split_tiles);
+  }
+  if (f.nsplit > 1) {
+    TfTraceScope tr("score_join_kernel", st);
+    hipLaunchKernelGGL(score_join_kernel<F32>, dim3((unsigned)(((long long)a->B * a->H * a->Sq + 3) / 4)), dim3(256), 0, st, *a, f.nsplit);
+  }
+  return (int)hipGetLastError();
+}
+
+template <bool F32, int HDP> int launch_bwd(const TfScoreAttnArgs* a, hipStream_t st) {
+  const double fl = 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D;
+  const int nqb = (a->Sq + 127) / 128, nkb = (a->Sk + 127) / 128;
+  const size_t lds = 64 * STile<F32, HDP>::STR + 32 * 16;
+  if (nqb > 0) {
+    allow_lds(score_dq_kernel<F32, HDP>, lds);
+    TfTraceScope tr(F32 ? "score_dq_kernel<fp32>" : "score_dq_kernel<bf16>", st, 1.5 * fl);
+    hipLaunchKernelGGL((score_dq_kernel<F32, HDP>), dim3(a->B * a->H * nqb), dim3(256), lds, st, *a, nqb);
+  }
+  if (a->dslopes != nullptr) {
+    TfTraceScope tr("score_dslope_kernel", st);
+    hipLaunchKernelGGL(score_dslope_kernel, dim3(a->H), dim3(256), 0, st, (const float*)a->dslope_rows, a->dslopes, a->B, a->H, a->Sq);
+  }
+  if (nkb > 0) {
+    TfTraceScope tr(F32 ? "score_dkv_kernel<fp32>" : "score_dkv_kernel<bf16>", st, 2.0 * fl);
+    auto go = [&](auto kern) {
+      allow_lds(kern, lds);
+      hipLaunchKernelGGL(kern, dim3(a->B * a->Hk * nkb), dim3(256), lds, st, *a, nkb);
+    };
+    if constexpr (HDP <= (F32 ? 128 : 192)) go(score_dkv_kernel<F32, HDP, 2>);
+    else { go(score_dkv_kernel<F32, HDP, 0>); go(score_dkv_kernel<F32, HDP, 1>); }
+  }
+  return (int)hipGetLastError();
+}
+
+template <class Fn> int by_head_dim(const TfScoreAttnArgs* a, Fn&& fn) {
+  auto pick = [&](auto f32) {
+    switch (hdp_of(a->D)) {
+      case 32: return fn(f32, std::integral_constant<int, 32>{});
+      case 64: return fn(f32, std::integral_constant<int, 64>{});
+      case 96: return fn(f32, std::integral_constant<int, 96>{});
+      case 128: return fn(f32, std::integral_constant<int, 128>{});
+      case 192: return fn(f32, std::integral_constant<int, 192>{});
+      default: return fn(f32, std::integral_constant<int, 256>{});
+    }
+  };
+  return a->is_f32 ? pick(std::true_type{}) : pick(std::false_type{});
+}
+
+}  // namespace
+
+// bytes of TfScoreAttnArgs.work for the forward; the backward needs none
+extern "C" size_t tf_score_attn_work(const TfScoreAttnArgs* a) {
+  if (check(a) != 0 || a->B == 0 || a->Sq == 0) return 0;
+  const FwdPlan f = fwd_plan(a);
+  return f.nsplit > 1 ? (size_t)f.nsplit * a->B * a->H * a->Sq * (a->D + 2) * sizeof(float) : 0;
+}
+
+extern "C" int tf_launch_score_fwd(const TfScoreAttnArgs* a, hipStream_t st) {
+  const int rc = check(a);
+  if (rc != 0) return rc;
+  if (a->B == 0 || a->Sq == 0) return 0;
+  const int e = a->is_f32 ? 4 : 2;
+  if (a->q == nullptr || a->out == nullptr || (a->Sk > 0 && (a->k == nullptr || a->v == nullptr))) return -6;
+  if (!aligned(a->q, a->q_sb, a->q_ss, a->q_sh, e) || !aligned(a->k, a->k_sb, a->k_ss, a->k_sh, e) || !aligned(a->v, a->v_sb, a->v_ss, a->v_sh, e) ||
+      !aligned(a->out, 0, 0, 0, e)) return -7;
+  const size_t need = tf_score_attn_work(a);
+  if (need > 0 && (a->work == nullptr || a->work_bytes < need || ((uintptr_t)a->work & 15) != 0)) return -8;
+  return by_head_dim(a, [&](auto f32, auto hdp) { return launch_fwd<decltype(f32)::value, decltype(hdp)::value>(a, st); });
+}
+
+extern "C" int tf_launch_score_bwd(const TfScoreAttnArgs* a, hipStream_t st) {
+  const int rc = check(a);
+  if (rc != 0) return rc;
+  if (a->B == 0) {
+    if (a->dslopes != nullptr) hipLaunchKernelGGL(score_dslope_kernel, dim3(a->H), dim3(256), 0, st, (const float*)nullptr, a->dslopes, 0, a->H, 0);
+    return (int)hipGetLastError();
+  }
+  const int e = a->is_f32 ? 4 : 2;
+  if (a->Sq > 0 && (a->q == nullptr || a->out == nullptr || a->dout == nullptr || a->dq == nullptr || a->lse == nullptr || a->delta == nullptr)) return -6;
+  if (a->Sk > 0 && (a->k == nullptr || a->v == nullptr || a->dk == nullptr || a->dv == nullptr)) return -6;
+  if (a->dslopes != nullptr && (a->slopes == nullptr || (a->Sq > 0 && a->dslope_rows == nullptr))) return -6;
+  if (!aligned(a->q, a->q_sb, a->q_ss, a->q_sh, e) || !aligned(a->k, a->k_sb, a->k_ss, a->k_sh, e) || !aligned(a->v, a->v_sb, a->v_ss, a->v_sh, e) ||
+      !aligned(a->dout, a->do_sb, a->do_ss, a->do_sh, e) || !aligned(a->out, 0, 0, 0, e) || !aligned(a->dq, 0, 0, 0, e) ||
+      !aligned(a->dk, 0, 0, 0, e) || !aligned(a->dv, 0, 0, 0, e)) return -7;
+  return by_head_dim(a, [&](auto f32, auto hdp) { return launch_bwd<decltype(f32)::value, decltype(hdp)::value>(a, st); });
+}

@@ -551,6 +551,18 @@ int tf_lm_pool_fwd(const TfLmPoolArgs* a, tf_stream_t s) { TF_TRY(tf_launch_lm_p
 int tf_lm_pool_bwd(const TfLmPoolArgs* a, tf_stream_t s) { TF_TRY(tf_launch_lm_pool_bwd(a, (hipStream_t)s), "tf_lm_pool_bwd"); return 0; }
 int tf_sumsq(const float* x, long long n, float* out, tf_stream_t s) { TF_TRY(tf_launch_sumsq(x, n, out, (hipStream_t)s), "tf_sumsq"); return 0; }
 int tf_sumsq_set(const float* x, long long n, float* out, tf_stream_t s) { TF_TRY(tf_launch_sumsq_ex(x, n, out, 0, (hipStream_t)s), "tf_sumsq_set"); return 0; }
+int tf_rotary(const TfRotaryArgs* a, tf_stream_t s) { TF_WRAP("tf_rotary", tf_launch_rotary(a, (hipStream_t)s)); }
+int tf_score_attn_fwd(const TfScoreAttnArgs* a, tf_stream_t s) { TF_WRAP("tf_score_attn_fwd", tf_launch_score_fwd(a, (hipStream_t)s)); }
+int tf_score_attn_bwd(const TfScoreAttnArgs* a, tf_stream_t s) { TF_WRAP("tf_score_attn_bwd", tf_launch_score_bwd(a, (hipStream_t)s)); }
+int tf_grad_clip(const TfGradClipArgs* a, tf_stream_t s) {
+  if (a == nullptr) return fail(-1, "tf_grad_clip");
+  try {
+    TF_TRY(tf_launch_grad_clip(a, (hipStream_t)s), "tf_grad_clip");
+  } catch (const std::exception&) {            // host memory for the overlap check
+    return fail(-20, "tf_grad_clip");
+  }
+  return 0;
+}
 int tf_sq_loss_fwd(const TfSqLossArgs* a, tf_stream_t s) {
   if (a == nullptr) return fail(-1, "tf_sq_loss_fwd");
   TF_TRY(tf_launch_sq_loss(a, 0, (hipStream_t)s), "tf_sq_loss_fwd");

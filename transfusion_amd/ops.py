@@ -4,6 +4,7 @@ given CPU tensors -- there is no CPU path.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -39,6 +40,14 @@ except AttributeError:               # (a torch build without the private entry 
 
     def _cur_device():
         return 0
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(dev):
+    """Makes ``dev`` current for a launch when it is not (the library launches on the current device's current stream)."""
+    return _HERE if dev.index == _cur_device() else torch.cuda.device(dev)
 
 
 def _is_f32(t) -> int:

@@ -34,6 +34,53 @@ def radam_schedule(step: int, beta1: float, beta2: float, degenerated_to_sgd: bo
     return n_sma, -1.0, 0
 
 
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0):
+    """``torch.nn.utils.clip_grad_norm_`` on the device, over any number of separate gradient tensors (tf_grad_clip): returns the norm over
+    all of them as a 0-d fp32 device tensor (no host synchronisation) and multiplies every gradient by ``min(1, max_norm / (norm + 1e-6))``
+    in place.  ``max_norm=inf`` only measures.  ``norm_type``: 2 or inf.  Gradients are fp32 or bf16 tensors (mixed freely) on one device that
+    fill their memory without gaps, in any order of their axes; a parameter listed twice counts once, parameters without a gradient are
+    skipped.  A norm that is not finite behaves as in torch: an infinite one zeroes what is finite, a NaN spreads."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    max_norm, norm_type = float(max_norm), float(norm_type)
+    if norm_type not in (2.0, math.inf):
+        raise L.TfError(f"clip_grad_norm_: norm_type {norm_type} is not supported (2 or inf)")
+    if not max_norm >= 0.0:
+        raise L.TfError(f"clip_grad_norm_: max_norm {max_norm} must not be negative")
+    grads, seen = [], set()
+    for p in parameters:
+        g = p.grad
+        if g is None or id(g) in seen:
+            continue
+        seen.add(id(g))
+        grads.append(g)
+    if not grads:
+        return torch.tensor(0.0)
+    dev = grads[0].device
+    n = len(grads)
+    ptrs, lens, bf = (L.C.c_void_p * n)(), (L.C.c_longlong * n)(), (L.C.c_int * n)()
+    for i, g in enumerate(grads):
+        if not g.is_cuda:
+            ops._require_cuda(g)
+        if g.device != dev or g.layout != torch.strided:
+            raise L.TfError("clip_grad_norm_: dense gradients on one device expected")
+        bf[i] = 1 - ops._is_f32(g)
+        if not g.is_contiguous() and not torch.ops.aten.is_non_overlapping_and_dense(g):
+            raise L.TfError(f"clip_grad_norm_: a gradient of shape {tuple(g.shape)} and strides {g.stride()} has gaps or overlaps itself")
+        ptrs[i], lens[i] = g.data_ptr(), g.numel()
+    parts = L.load().tf_grad_clip_parts(lens, n)
+    work = torch.empty(max(parts, 1), dtype=torch.float64, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    clip = max_norm < math.inf
+    a = L.TfGradClipArgs(grads=L.C.addressof(ptrs), n=L.C.addressof(lens), is_bf16=L.C.addressof(bf), count=n, norm_type=int(norm_type == math.inf),
+                         clip=int(clip), max_norm=max_norm if clip else 0.0, norm=L.ptr(norm), work=L.ptr(work), parts=parts)
+    with ops.on_device(dev):
+        L.call("tf_grad_clip", a, ops._stream())
+    if clip:
+        torch._C._increment_version(grads)          # written through raw pointers
+    return norm
+
+
 class FusedRAdam(torch.optim.Optimizer):
     """``step(grad_scale=..., sumsq=..., clip=...)``: the gradient is multiplied by ``grad_scale`` first (1 / world size, loss
     scale) and, with ``sumsq`` + ``clip``, by torch's clip_grad_norm_ coefficient computed on the device."""
