@@ -31,12 +31,13 @@ def _heads(name, t, like=None):
 
 
 def _rows(t):
-    """``t`` itself if its channels are contiguous and every row starts on 16 bytes, else a contiguous copy."""
+    """``t`` itself if its channels are contiguous, every row starts on 16 bytes and the rows lie within 16 MiB of each other (64 of them
+    are addressed with 32-bit offsets), else a contiguous copy."""
     e = t.element_size()
     if t.numel() == 0:
         return t
     ok = (t.shape[3] == 1 or t.stride(3) == 1) and t.data_ptr() % 16 == 0
-    ok = ok and all(t.shape[i] == 1 or t.stride(i) * e % 16 == 0 for i in range(3))
+    ok = ok and all(t.shape[i] == 1 or t.stride(i) * e % 16 == 0 for i in range(3)) and t.stride(1) * e < 1 << 24
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 

@@ -259,6 +259,351 @@ __global__ __launch_bounds__(256, 1) void score_fwd_kernel(const TfScoreAttnArgs
   if (h == 0 && a.lse != nullptr) a.lse[row] = l_tot == 0.f ? INFINITY : m_run + log2f(l_tot);
 }
 
+// ================================================================================================
+// forward, bf16
+// ================================================================================================
+// LDS tiles of the bf16 kernels: 64 rows of HDP channels at a stride of an ODD multiple of 64 bytes, 16-byte piece ^= (row >> 2) & 3:
+// four consecutive rows start 16 banks apart in some order, so row reads (ds_read_b128) and transposed reads (ds_read_b64_tr_b16) are
+// both free of conflicts -- at the smallest such stride (192 bytes for 64 channels, 448 for 192).
+template <int HDP> struct SGeo {
+  static constexpr int STR = ((HDP * 2 + 63) / 64 | 1) * 64;
+  static constexpr int KS = HDP / 16, DB = HDP / 32, TILE = 64 * STR;
+};
+// LDS-DMA of a 64-row tile by four waves: the image is linear in the lane, so the layout lives on the source side.  Pieces at or beyond D
+// get an offset behind the buffer's end and arrive as zeros, as do rows beyond its last.
+template <int HDP> struct SDma {
+  static constexpr int T = SGeo<HDP>::STR, NI = 64 * T / 4096;
+  static constexpr unsigned OUT = 0x7fffff00u;
+  unsigned off[NI], rb;       // offsets for rows of rb bytes; a matrix with other rows has them formed where it is read
+  int wave, lane;
+  __device__ __forceinline__ unsigned offset(int i, unsigned row_bytes, int D) const {
+    const int pos = (wave * NI + i) * 1024 + lane * 16, r = pos / T, cp = (pos % T) >> 4, c = cp ^ ((r >> 2) & 3);
+    return cp >= HDP / 8 || c * 8 >= D ? OUT : (unsigned)r * row_bytes + c * 16;
+  }
+  __device__ __forceinline__ SDma(int wave_, int lane_, unsigned row_bytes, int D) : rb(row_bytes), wave(wave_), lane(lane_) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) off[i] = offset(i, row_bytes, D);
+  }
+  __device__ __forceinline__ int row(int i) const { return ((wave * NI + i) * 1024 + lane * 16) / T; }
+  // rows row0 .. of the matrix at base, row_end excluded; doc != null: rows of negative documents are zeros too (few tiles hold any)
+  __device__ __forceinline__ void issue(const char* base, unsigned row_bytes, int row0, int row_end, int D, const int* doc, unsigned char* tile) const {
+    const int n = min(64, row_end - row0);
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(base + (long long)row0 * row_bytes), 0, (int)((unsigned)(n - 1) * row_bytes + D * 2), 0x00020000);
+    if (doc == nullptr && row_bytes == rb) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TF_LDS_PTR(tile + (wave * NI + i) * 1024), 16, (int)off[i], 0, 0, 0);
+    } else {
+      for (int i = 0; i < NI; ++i) {
+        const unsigned o = doc != nullptr && doc[row0 + min(row(i), n - 1)] < 0 ? OUT : offset(i, row_bytes, D);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TF_LDS_PTR(tile + (wave * NI + i) * 1024), 16, (int)o, 0, 0, 0);
+      }
+    }
+  }
+};
+// per-lane LDS addresses of row fragments (32 rows x 16 channels) and transposed fragments of such a tile; see attn_common.h FragAddr
+template <int HDP> struct SAddr {
+  static constexpr int T = SGeo<HDP>::STR;
+  unsigned row_e, row_o, tr_a, tr_b;
+  __device__ __forceinline__ SAddr(unsigned tile, int lane) {
+    const int r = lane & 31, x = (r >> 2) & 3, hh = lane >> 5;
+    row_e = tile + r * T + ((hh ^ x) << 4);
+    row_o = tile + r * T + (((2 + hh) ^ x) << 4);
+    const int li = lane & 15, q4 = li >> 2, p = li & 3, cb = (lane >> 4) & 1, low2 = 2 * cb + (p >> 1);
+    tr_a = tile + (4 * hh + q4) * T + ((low2 ^ hh) << 4) + (p & 1) * 8;
+    tr_b = tile + (4 * hh + q4 + 8) * T + ((low2 ^ (hh + 2)) << 4) + (p & 1) * 8;
+  }
+  template <int ROW0, int KS> __device__ __forceinline__ u32x4 row() const { return rd128_asm<ROW0 * T + 64 * (KS >> 1)>((KS & 1) ? row_o : row_e); }
+  template <int KROW0, int COL0> __device__ __forceinline__ void tr(u64& a, u64& b) const {
+    a = tr_read_asm<KROW0 * T + 2 * COL0>(tr_a);
+    b = tr_read_asm<KROW0 * T + 2 * COL0>(tr_b);
+  }
+};
+
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ u64 scalar64(u64 v) {
+  return ((u64)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)v);
+}
+// the keys of a tile (document of key kv0 + lane in kd) that belong to this lane's document: one ballot per document among the lanes
+__device__ __forceinline__ u64 doc_bits(int qd, int kd) {
+  u64 bits = 0ull, todo = ~0ull;
+  while (todo != 0ull) {
+    const int d = __builtin_amdgcn_readlane(qd, __builtin_ctzll(todo));
+    const u64 hit = __ballot(kd == d && kd >= 0);
+    const bool mine = qd == d;
+    if (mine) bits = hit;
+    todo &= ~__ballot(mine);
+  }
+  return bits;
+}
+
+// 64-tile chunks of a row of 64-item tiles against a range of documents [dmin, dmax] of the other side: which tiles hold an item inside the
+// range (vis), only items of the range's one document (full), an item of a negative document (neg).  Called by all four waves.
+struct DocChunk { u64 vis, full, neg; };
+__device__ __forceinline__ DocChunk doc_chunk(const int* __restrict__ doc, int tile0, int tiles, int items, int dmin, int dmax, u64 (*sh)[3], int wave, int lane) {
+  u64 vis = 0ull, full = 0ull, neg = 0ull;
+#pragma unroll 4
+  for (int s = 0; s < 16; ++s) {
+    const int t = s * 4 + wave;
+    if (t >= tiles) break;
+    const int i = (tile0 + t) * 64 + lane;
+    const bool in = i < items;
+    const int d = in ? doc[i] : -1;
+    if (__any(d >= dmin && d <= dmax)) vis |= 1ull << t;
+    if (__all(!in || d == dmin) && dmin == dmax) full |= 1ull << t;
+    if (__any(in && d < 0)) neg |= 1ull << t;
+  }
+  __syncthreads();
+  if (lane == 0) { sh[wave][0] = vis; sh[wave][1] = full; sh[wave][2] = neg; }
+  __syncthreads();
+  DocChunk c;
+  c.vis = scalar64(sh[0][0] | sh[1][0] | sh[2][0] | sh[3][0]);
+  c.full = scalar64(sh[0][1] | sh[1][1] | sh[2][1] | sh[3][1]);
+  c.neg = scalar64(sh[0][2] | sh[1][2] | sh[2][2] | sh[3][2]);
+  return c;
+}
+// the tiles t of [t_lo, t_end) a workgroup visits, in order: all of them, or, with documents, those whose range meets the workgroup's own
+template <bool DOC> struct TileWalk {
+  const int* doc;
+  int t_end, items, dmin, dmax, base;       // base: first tile of the chunk in hand
+  DocChunk c;
+  bool full, neg;
+  __device__ __forceinline__ int chunk_from(int t, u64 (*sh)[3], int wave, int lane) {
+    for (base = t; base < t_end; base += 64) {
+      c = doc_chunk(doc, base, min(64, t_end - base), items, dmin, dmax, sh, wave, lane);
+      if (c.vis != 0ull) return take();
+    }
+    return -1;
+  }
+  __device__ __forceinline__ int take() {
+    const int i = __builtin_ctzll(c.vis);
+    c.vis &= c.vis - 1ull;
+    full = (c.full >> i) & 1ull;
+    neg = (c.neg >> i) & 1ull;
+    return base + i;
+  }
+  __device__ __forceinline__ int first(int t_lo, u64 (*sh)[3], int wave, int lane) {
+    full = true;
+    neg = false;
+    if (!DOC) return t_lo < t_end ? t_lo : -1;
+    return dmin > dmax ? -1 : chunk_from(t_lo, sh, wave, lane);
+  }
+  __device__ __forceinline__ int next(int t, u64 (*sh)[3], int wave, int lane) {
+    if (!DOC) return t + 1 < t_end ? t + 1 : -1;
+    return c.vis != 0ull ? take() : chunk_from(base + 64, sh, wave, lane);
+  }
+};
+
+// 128 queries a workgroup (32 a wave, on the lane), 64-key tiles by LDS-DMA: V(t) travels under S(t) and the softmax, K(t + 1) under PV(t).
+// Two workgroups a CU (heads <= 192) hide the barriers of one behind the matrix work of the other.
+// DOC: documents are given.
+template <int HDP, bool DOC>
+__global__ __launch_bounds__(256, (HDP <= 192 ? 2 : 1)) void score_fwd16_kernel(const TfScoreAttnArgs a, int nqb, int nsplit, int split_tiles) {
+  using G = SGeo<HDP>;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  unsigned char* kt = smem;
+  unsigned char* vt = smem + G::TILE;
+  u64 (*dsh)[3] = (u64 (*)[3])(smem + 2 * G::TILE);
+  int* rsh = (int*)(smem + 2 * G::TILE + 96);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int logical = xcd_remap(blockIdx.x, gridDim.x);
+  const int split = logical % nsplit, t1 = logical / nsplit;
+  const int qb = nqb - 1 - t1 % nqb, bh = t1 / nqb, b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.Hk);
+  const char* qbase = (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * 2;
+  const char* kbase = (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * 2;
+  const char* vbase = (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * 2;
+  const unsigned krb = (unsigned)a.k_ss * 2, vrb = (unsigned)a.v_ss * 2;
+  const int* kdoc = DOC ? a.k_doc + (size_t)b * a.Sk : nullptr;
+  const SMod m = smod(a, head);
+  const int p0 = q_pos0(a, b), pfx = prefix_of(a, b);
+  const int w0 = qb * 128 + wave * 32, i = w0 + (lane & 31), ic = min(i, a.Sq - 1);
+  const int qd = DOC ? a.q_doc[(size_t)b * a.Sq + ic] : 0;
+  const bool live = i < a.Sq && qd >= 0, wave_live = w0 < a.Sq;
+  const int p = p0 + i;
+  const int lim = a.causal ? min(max(p, pfx - 1), a.Sk - 1) : a.Sk - 1;
+  const int lim_lo = a.causal ? min(max(p0 + w0, pfx - 1), a.Sk - 1) : a.Sk - 1;                       // of the wave's first row
+  const int lim_hi = a.causal ? min(max(p0 + min(w0 + 31, a.Sq - 1), pfx - 1), a.Sk - 1) : a.Sk - 1;   // of its last
+  const int hi = a.causal ? min(max(p0 + min(qb * 128 + 127, a.Sq - 1) + 1, pfx), a.Sk) : a.Sk;
+  TileWalk<DOC> walk{kdoc, min((max(hi, 0) + 63) / 64, (split + 1) * split_tiles), a.Sk, 0, 0, 0, {}, true, false};
+  if (DOC) {                  // the documents of the block's rows
+    const int lo = wave_min_i(live ? qd : 0x7fffffff), up = -wave_min_i(live ? -qd : 0x7fffffff);
+    if (lane == 0) { rsh[wave] = lo; rsh[4 + wave] = up; }
+    __syncthreads();
+    walk.dmin = __builtin_amdgcn_readfirstlane(min(min(rsh[0], rsh[1]), min(rsh[2], rsh[3])));
+    walk.dmax = __builtin_amdgcn_readfirstlane(max(max(rsh[4], rsh[5]), max(rsh[6], rsh[7])));
+  }
+  u32x4 qf[G::KS];
+#pragma unroll
+  for (int ks = 0; ks < G::KS; ++ks) qf[ks] = gfrag<false>(qbase + (long long)ic * a.q_ss * 2, ks, h, a.D, live).v;
+  f32x16 o[G::DB];
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m_run = S_NEG, l_run = 0.f;
+  const bool changed = m.capl != 0.f || m.slope2 != 0.f || !(m.sc > 0.f);      // else the scale rides in the exponent's FMA
+  const float scf = changed ? 1.0f : m.sc;
+  const SAddr<HDP> fk(lds_addr_of(kt), lane), fv(lds_addr_of(vt), lane);
+  const SDma<HDP> dma(wave, lane, krb, a.D);
+  int t = walk.first(split * split_tiles, dsh, wave, lane);
+  bool full = walk.full, neg = walk.neg;
+  int kd_n = 0;
+  if (t >= 0) {
+    if (DOC) kd_n = t * 64 + lane < a.Sk ? kdoc[t * 64 + lane] : -1;
+    dma.issue(kbase, krb, t * 64, hi, a.D, DOC && neg ? kdoc : nullptr, kt);
+  }
+  while (t >= 0) {
+    const int kv0 = t * 64;
+    const bool full_t = full && kv0 + 63 <= lim_lo, work = wave_live && kv0 <= lim_hi;
+    const int kd = kd_n;
+    dma_wait_barrier();                   // K(t) is there; every wave is done with V(t - 1)
+    dma.issue(vbase, vrb, kv0, hi, a.D, DOC && neg ? kdoc : nullptr, vt);
+    unsigned pk[2][8];
+    if (work) {
+      f32x16 st[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[kb][r] = 0.f;
+      {
+        constexpr int NF = 2 * G::KS, PF = 3;
+        u32x4 fr[NF];
+        static_for<(PF < NF ? PF : NF)>([&](auto I) { fr[I] = fk.template row<(I & 1) * 32, (I >> 1)>(); });
+        static_for<NF>([&](auto I) {
+          constexpr int x = I, nx = x + PF;
+          if constexpr (nx < NF) fr[nx] = fk.template row<(nx & 1) * 32, (nx >> 1)>();
+          lgkm_wait<(NF - 1 - x < PF ? NF - 1 - x : PF)>(fr[x]);
+          st[x & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(fr[x]), as_bf16x8(qf[x >> 1]), st[x & 1], 0, 0, 0);
+        });
+      }
+      if (changed) {                      // (workgroup-uniform)
+        if (m.capl != 0.f) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[kb][r] = m.capl * tanh_of<false>(st[kb][r] * m.sc);
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[kb][r] *= m.sc;
+        }
+        if (m.slope2 != 0.f) {
+          const float pd = (float)(p - kv0 - 4 * h);
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[kb][r] -= m.slope2 * fabsf(pd - (float)(kb * 32 + (r & 3) + 8 * (r >> 2)));
+        }
+      }
+      if (!full_t) {
+        const int n = lim - kv0 + 1;
+        u64 bits = n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1ull;
+        if (DOC) bits &= doc_bits(qd, kd);
+        bits >>= 4 * h;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (!((bits >> (kb * 32 + (r & 3) + 8 * (r >> 2))) & 1ull)) st[kb][r] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[kb][r]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * scf;
+      const bool need = mx - m_run > RESCALE_THR;        // per row; the wave only skips the multiplication when no row needs it
+      if (__any(need)) {
+        const float m_new = need ? fmaxf(m_run, mx) : m_run, alpha = need ? fast_exp2(m_run - m_new) : 1.0f;
+        m_run = m_new;
+        l_run *= alpha;
+#pragma unroll
+        for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+      }
+      float ps0 = 0.f, ps1 = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float e0 = fast_exp2(fmaf(st[kb][r], scf, -m_run)), e1 = fast_exp2(fmaf(st[kb][r + 1], scf, -m_run));
+          ps0 += e0;
+          ps1 += e1;
+          pk[kb][r >> 1] = cvt_pk_bf16(e0, e1);
+        }
+      l_run += ps0 + ps1;
+    }
+    const int tn = walk.next(t, dsh, wave, lane);        // (may scan documents, with barriers of its own: all waves take part)
+    full = walk.full;
+    neg = walk.neg;
+    dma_wait_barrier();                   // V(t) is there; every wave is done with K(t)
+    if (tn >= 0) {
+      if (DOC) kd_n = tn * 64 + lane < a.Sk ? kdoc[tn * 64 + lane] : -1;
+      dma.issue(kbase, krb, tn * 64, hi, a.D, DOC && neg ? kdoc : nullptr, kt);
+    }
+    if (work) {
+      constexpr int NF = 4 * G::DB, PF = 2;
+      u64 fa[NF], fb[NF];
+      bf16x8 pf[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int kb = g >> 1, s4 = 4 * (g & 1);
+        pf[g] = as_bf16x8(u32x4{pk[kb][s4], pk[kb][s4 + 1], pk[kb][s4 + 2], pk[kb][s4 + 3]});
+      }
+      static_for<PF>([&](auto I) { fv.template tr<(I / G::DB) * 16, (I % G::DB) * 32>(fa[I], fb[I]); });
+      static_for<NF>([&](auto I) {
+        constexpr int x = I, nx = x + PF;
+        if constexpr (nx < NF) fv.template tr<(nx / G::DB) * 16, (nx % G::DB) * 32>(fa[nx], fb[nx]);
+        lgkm_wait<2 * (NF - 1 - x < PF ? NF - 1 - x : PF)>(fa[x], fb[x]);
+        o[x % G::DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join_tr64(fa[x], fb[x]), pf[x / G::DB], o[x % G::DB], 0, 0, 0);
+      });
+    }
+    t = tn;
+  }
+  const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+  const long long rows = (long long)a.B * a.H * a.Sq, row = (long long)bh * a.Sq + i;
+  const bool none = !live || l_tot == 0.f;
+  if (nsplit > 1) {
+    if (i >= a.Sq) return;
+    float* po = (float*)a.work + ((long long)split * rows + row) * a.D;
+    float* pml = (float*)a.work + (long long)nsplit * rows * a.D + ((long long)split * rows + row) * 2;
+#pragma unroll
+    for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = d * 32 + 8 * g + 4 * h;
+        if (c < a.D) *(f32x4*)(po + c) = none ? f32x4{0, 0, 0, 0} : f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+      }
+    if (h == 0) { pml[0] = none ? S_NEG : m_run; pml[1] = none ? 0.f : l_tot; }
+    return;
+  }
+  const float inv = 1.0f / l_tot;
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = none ? 0.f : o[d][r] * inv;
+  u16* orow = (u16*)a.out + (((long long)b * a.Sq + ic) * a.H + head) * a.D;
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int pr = 0; pr < 2; ++pr) {      // lane and lane ^ 32 hold 4 channels each of every 8: they swap one group of a pair, then 16-byte stores
+      const int ge = 2 * pr, go = 2 * pr + 1;
+      const unsigned e0 = pack2bf(o[d][4 * ge] , o[d][4 * ge + 1]), e1 = pack2bf(o[d][4 * ge + 2] , o[d][4 * ge + 3]);
+      const unsigned o0 = pack2bf(o[d][4 * go] , o[d][4 * go + 1]), o1 = pack2bf(o[d][4 * go + 2] , o[d][4 * go + 3]);
+      const u32x2 s0 = __builtin_amdgcn_permlane32_swap(e0, o0, false, false);
+      const u32x2 s1 = __builtin_amdgcn_permlane32_swap(e1, o1, false, false);
+      const int c = d * 32 + 8 * (2 * pr + h);
+      if (i < a.Sq && c < a.D) *(u32x4*)(orow + c) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+    }
+  if (i < a.Sq && h == 0 && a.lse != nullptr) a.lse[row] = none ? INFINITY : m_run + log2f(l_tot);
+}
+
 // joins the parts of a split forward: one wave a row, four channels a lane
 template <bool F32> __global__ __launch_bounds__(256) void score_join_kernel(const TfScoreAttnArgs a, int nsplit) {
   const long long rows = (long long)a.B * a.H * a.Sq, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -556,18 +901,22 @@ int check(const TfScoreAttnArgs* a) {
   if (blocks > 0x3fffff || (long long)a->Sq + a->Sk > (1ll << 30)) return -5;
   return 0;
 }
+// (64 rows of a tile are addressed with 32-bit offsets)
 bool aligned(const void* p, long long sb, long long ss, long long sh, int e) {
-  return (((uintptr_t)p) & 15) == 0 && sb * e % 16 == 0 && ss * e % 16 == 0 && sh * e % 16 == 0;
+  return (((uintptr_t)p) & 15) == 0 && sb >= 0 && ss >= 0 && sh >= 0 && ss < (1ll << 30) / 64 / e && sb * e % 16 == 0 && ss * e % 16 == 0 && sh * e % 16 == 0;
 }
 
 template <bool F32, int HDP> int launch_fwd(const TfScoreAttnArgs* a, hipStream_t st) {
-  constexpr int KT = F32 ? 32 : 64;
   const FwdPlan f = fwd_plan(a);
-  const size_t lds = 2 * KT * STile<F32, HDP>::STR + KT * 4;
-  allow_lds(score_fwd_kernel<F32, HDP>, lds);
   {
-    TfTraceScope tr(F32 ? "score_fwd_kernel<fp32>" : "score_fwd_kernel<bf16>", st, 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D);
-    hipLaunchKernelGGL((score_fwd_kernel<F32, HDP>), dim3(a->B * a->H * f.nqb * f.nsplit), dim3(256), lds, st, *a, f.nqb, f.nsplit, f.split_tiles);
+    TfTraceScope tr(F32 ? "score_fwd_kernel" : "score_fwd16_kernel", st, 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D);
+    auto go = [&](auto kern, size_t lds) {
+      allow_lds(kern, lds);
+      hipLaunchKernelGGL(kern, dim3(a->B * a->H * f.nqb * f.nsplit), dim3(256), lds, st, *a, f.nqb, f.nsplit, f.split_tiles);
+    };
+    if constexpr (F32) go(score_fwd_kernel<true, HDP>, 2 * 32 * STile<true, HDP>::STR + 32 * 4);
+    else if (a->k_doc != nullptr) go(score_fwd16_kernel<HDP, true>, 2 * SGeo<HDP>::TILE + 128);
+    else go(score_fwd16_kernel<HDP, false>, 2 * SGeo<HDP>::TILE + 128);
   }
   if (f.nsplit > 1) {
     TfTraceScope tr("score_join_kernel", st);
