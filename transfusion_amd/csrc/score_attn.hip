@@ -134,6 +134,15 @@ __device__ __forceinline__ int q_pos0(const TfScoreAttnArgs& a, int b) {
 }
 __device__ __forceinline__ int prefix_of(const TfScoreAttnArgs& a, int b) { return a.prefix != nullptr ? min(max(a.prefix[b], 0), a.Sk) : 0; }
 
+// (by value: a bit cast of a vector's element in place takes the vector's first)
+__device__ __forceinline__ float f_of(unsigned u) { return __builtin_bit_cast(float, u); }
+// two values -> one register of bf16 in one instruction (spelt so that the compiler keeps the wait between an exponential and its use)
+__device__ __forceinline__ unsigned pk2(float lo, float hi) {
+  typedef __attribute__((ext_vector_type(2))) float f32x2;
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+  const f32x2 v = {lo, hi};
+  return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+}
 constexpr float S_NEG = -1.0e38f;          // the running maximum before the first visible key
 
 // ================================================================================================
@@ -535,7 +544,7 @@ __global__ __launch_bounds__(256, (HDP <= 192 ? 2 : 1)) void score_fwd16_kernel(
           const float e0 = fast_exp2(fmaf(st[kb][r], scf, -m_run)), e1 = fast_exp2(fmaf(st[kb][r + 1], scf, -m_run));
           ps0 += e0;
           ps1 += e1;
-          pk[kb][r >> 1] = cvt_pk_bf16(e0, e1);
+          pk[kb][r >> 1] = pk2(e0, e1);
         }
       l_run += ps0 + ps1;
     }
@@ -864,6 +873,396 @@ __global__ __launch_bounds__(256, 1) void score_dkv_kernel(const TfScoreAttnArgs
 }
 
 // ================================================================================================
+// backward, bf16
+// ================================================================================================
+// Two 32-row tiles that are used together (K and V, or Q and dO), staged as one image of 64 rows: waves 0 and 1 fetch the first matrix,
+// 2 and 3 the second.  Two images: the next pair travels under the whole of this one's work, one barrier a pair.
+template <int HDP> struct PairDma {
+  static constexpr int T = SGeo<HDP>::STR, NI = 64 * T / 4096, HALF = 32 * T, BUF = 64 * T;
+  unsigned off[NI];
+  int wave, lane;
+  __device__ __forceinline__ int row(int i) const { return ((wave & 1) * NI * 1024 + i * 1024 + lane * 16) / T; }
+  __device__ __forceinline__ PairDma(int wave_, int lane_, unsigned row_bytes, int D) : wave(wave_), lane(lane_) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int pos = (wave & 1) * NI * 1024 + i * 1024 + lane * 16, r = pos / T, cp = (pos % T) >> 4, c = cp ^ ((r >> 2) & 3);
+      off[i] = cp >= HDP / 8 || c * 8 >= D ? SDma<HDP>::OUT : (unsigned)r * row_bytes + c * 16;
+    }
+  }
+  // base, row_bytes: of the matrix this wave fetches.  Rows at or beyond row_end and (doc != null) rows of negative documents: zeros
+  __device__ __forceinline__ void issue(const char* base, unsigned row_bytes, int row0, int row_end, int D, const int* doc, unsigned char* image) const {
+    const int n = min(32, row_end - row0);
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(base + (long long)row0 * row_bytes), 0, (int)((unsigned)(n - 1) * row_bytes + D * 2), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      unsigned o = off[i];
+      if (doc != nullptr && doc[row0 + min(row(i), n - 1)] < 0) o = SDma<HDP>::OUT;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TF_LDS_PTR(image + (wave * NI + i) * 1024), 16, (int)o, 0, 0, 0);
+    }
+  }
+};
+// st += X . x and dp += Y . y of a pair image: row fragments PF ahead of their matrix instruction, the two accumulators in turn
+template <int HDP> __device__ __forceinline__ void pair_rows(const SAddr<HDP>& fx, const SAddr<HDP>& fy, const u32x4 (&x)[HDP / 16], const u32x4 (&y)[HDP / 16],
+                                                             f32x16& st, f32x16& dp) {
+  constexpr int NF = 2 * (HDP / 16), PF = 4;
+  u32x4 fr[NF];
+  static_for<PF>([&](auto I) { if constexpr (I & 1) fr[I] = fy.template row<0, (I >> 1)>(); else fr[I] = fx.template row<0, (I >> 1)>(); });
+  static_for<NF>([&](auto I) {
+    constexpr int i = I, nx = i + PF;
+    if constexpr (nx < NF) { if constexpr (nx & 1) fr[nx] = fy.template row<0, (nx >> 1)>(); else fr[nx] = fx.template row<0, (nx >> 1)>(); }
+    lgkm_wait<(NF - 1 - i < PF ? NF - 1 - i : PF)>(fr[i]);
+    if constexpr (i & 1) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(fr[i]), as_bf16x8(y[i >> 1]), dp, 0, 0, 0);
+    else st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(fr[i]), as_bf16x8(x[i >> 1]), st, 0, 0, 0);
+  });
+}
+template <int HDP> __device__ __forceinline__ void one_rows(const SAddr<HDP>& fx, const u32x4 (&x)[HDP / 16], f32x16& st) {
+  constexpr int NF = HDP / 16, PF = NF < 4 ? NF : 4;
+  u32x4 fr[NF];
+  static_for<PF>([&](auto I) { fr[I] = fx.template row<0, I>(); });
+  static_for<NF>([&](auto I) {
+    constexpr int i = I, nx = i + PF;
+    if constexpr (nx < NF) fr[nx] = fx.template row<0, nx>();
+    lgkm_wait<(NF - 1 - i < PF ? NF - 1 - i : PF)>(fr[i]);
+    st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(fr[i]), as_bf16x8(x[i]), st, 0, 0, 0);
+  });
+}
+// acc[channel][lane] += sum over the 32 rows of a tile of tile[row][channel] * p[row]; p: 16 values packed as they lie in the accumulator
+template <int HDP> __device__ __forceinline__ void tile_t(const SAddr<HDP>& f, const unsigned (&p)[8], f32x16 (&acc)[HDP / 32]) {
+  constexpr int DB = HDP / 32, NF = 2 * DB, PF = 2;
+  u64 fa[NF], fb[NF];
+  static_for<PF>([&](auto I) { f.template tr<(I / DB) * 16, (I % DB) * 32>(fa[I], fb[I]); });
+  static_for<NF>([&](auto I) {
+    constexpr int i = I, nx = i + PF, s = 4 * (i / DB);
+    if constexpr (nx < NF) f.template tr<(nx / DB) * 16, (nx % DB) * 32>(fa[nx], fb[nx]);
+    lgkm_wait<2 * (NF - 1 - i < PF ? NF - 1 - i : PF)>(fa[i], fb[i]);
+    acc[i % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join_tr64(fa[i], fb[i]), as_bf16x8(u32x4{p[s], p[s + 1], p[s + 2], p[s + 3]}), acc[i % DB], 0, 0, 0);
+  });
+}
+template <int HDP> __device__ __forceinline__ SAddr<HDP> shifted(const SAddr<HDP>& f, unsigned bytes) {
+  SAddr<HDP> g = f;
+  g.row_e += bytes; g.row_o += bytes; g.tr_a += bytes; g.tr_b += bytes;
+  return g;
+}
+
+// [rows of a 32-row accumulator tile][channels] of one lane -> 16-byte stores (see the forward's epilogue)
+template <int DB> __device__ __forceinline__ void store_lane_row(u16* row, const f32x16 (&x)[DB], float scale, int h, int D, bool ok) {
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int pr = 0; pr < 2; ++pr) {
+      const int ge = 8 * pr, go = 8 * pr + 4;
+      const unsigned e0 = pk2(x[d][ge] * scale, x[d][ge + 1] * scale), e1 = pk2(x[d][ge + 2] * scale, x[d][ge + 3] * scale);
+      const unsigned o0 = pk2(x[d][go] * scale, x[d][go + 1] * scale), o1 = pk2(x[d][go + 2] * scale, x[d][go + 3] * scale);
+      const u32x2 s0 = __builtin_amdgcn_permlane32_swap(e0, o0, false, false);
+      const u32x2 s1 = __builtin_amdgcn_permlane32_swap(e1, o1, false, false);
+      const int c = d * 32 + 8 * (2 * pr + h);
+      if (ok && c < D) *(u32x4*)(row + c) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+    }
+}
+
+// body(FULL, CAP, SLP) with the flags (all uniform over the wave) as compile-time constants: the loops over a tile's scores stay free of
+// branches and of registers that only one of their forms needs
+template <class F> __device__ __forceinline__ void by_flags(bool full, bool cap, bool slp, F&& body) {
+  auto two = [&](auto FULL) {
+    if (cap) { if (slp) body(FULL, std::true_type{}, std::true_type{}); else body(FULL, std::true_type{}, std::false_type{}); }
+    else { if (slp) body(FULL, std::false_type{}, std::true_type{}); else body(FULL, std::false_type{}, std::false_type{}); }
+  };
+  if (full) two(std::true_type{}); else two(std::false_type{});
+}
+
+// One step of a walk over 64-item tiles in halves of 32 items.
+template <bool DOC> struct HalfWalk {
+  TileWalk<DOC> w;
+  int s, items;                           // s: the half in hand (items 32 s ..), -1 at the end
+  bool full, neg;
+  __device__ __forceinline__ void first(int s0, u64 (*sh)[3], int wave, int lane) {
+    const int t = w.first(s0 >> 1, sh, wave, lane);
+    s = t < 0 ? -1 : max(2 * t, s0);
+    if (s >= 0 && s * 32 >= items) s = -1;
+    full = w.full;
+    neg = w.neg;
+  }
+  __device__ __forceinline__ void next(u64 (*sh)[3], int wave, int lane) {
+    if (!(s & 1) && (s + 1) * 32 < items) { ++s; return; }
+    const int t = w.next(s >> 1, sh, wave, lane);
+    s = t < 0 ? -1 : 2 * t;
+    full = w.full;
+    neg = w.neg;
+  }
+};
+
+// dq: query on the lane, 128 queries a workgroup; also delta = rowsum(dO o) and the slopes' row sums
+template <int HDP, bool DOC>
+__global__ __launch_bounds__(256, (HDP <= 128 ? 2 : 1)) void score_dq16_kernel(const TfScoreAttnArgs a, int nqb) {
+  using G = SGeo<HDP>;
+  using PD = PairDma<HDP>;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  u64 (*dsh)[3] = (u64 (*)[3])(smem + 2 * PD::BUF);
+  int* rsh = (int*)(smem + 2 * PD::BUF + 96);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int logical = xcd_remap(blockIdx.x, gridDim.x);
+  const int qb = nqb - 1 - logical % nqb, bh = logical / nqb, b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.Hk);
+  const char* qbase = (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * 2;
+  // this wave's matrix of the pair: K (waves 0, 1) or V
+  const char* xbase = wave < 2 ? (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * 2
+                               : (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * 2;
+  const unsigned xrb = (unsigned)(wave < 2 ? a.k_ss : a.v_ss) * 2;
+  const int* kdoc = DOC ? a.k_doc + (size_t)b * a.Sk : nullptr;
+  const SMod m = smod(a, head);
+  const int p0 = q_pos0(a, b), pfx = prefix_of(a, b);
+  const int w0 = qb * 128 + wave * 32, i = w0 + (lane & 31), ic = min(i, a.Sq - 1);
+  const int qd = DOC ? a.q_doc[(size_t)b * a.Sq + ic] : 0;
+  const bool live = i < a.Sq && qd >= 0, wave_live = w0 < a.Sq;
+  const int p = p0 + i;
+  const int lim = a.causal ? min(max(p, pfx - 1), a.Sk - 1) : a.Sk - 1;
+  const int lim_lo = a.causal ? min(max(p0 + w0, pfx - 1), a.Sk - 1) : a.Sk - 1;
+  const int lim_hi = a.causal ? min(max(p0 + min(w0 + 31, a.Sq - 1), pfx - 1), a.Sk - 1) : a.Sk - 1;
+  const int hi = a.causal ? min(max(p0 + min(qb * 128 + 127, a.Sq - 1) + 1, pfx), a.Sk) : a.Sk;
+  HalfWalk<DOC> walk{{kdoc, (max(hi, 0) + 63) / 64, a.Sk, 0, 0, 0, {}, true, false}, -1, max(hi, 0), true, false};
+  if (DOC) {
+    const int lo = wave_min_i(live ? qd : 0x7fffffff), up = -wave_min_i(live ? -qd : 0x7fffffff);
+    if (lane == 0) { rsh[wave] = lo; rsh[4 + wave] = up; }
+    __syncthreads();
+    walk.w.dmin = __builtin_amdgcn_readfirstlane(min(min(rsh[0], rsh[1]), min(rsh[2], rsh[3])));
+    walk.w.dmax = __builtin_amdgcn_readfirstlane(max(max(rsh[4], rsh[5]), max(rsh[6], rsh[7])));
+  }
+  walk.first(0, dsh, wave, lane);
+  const PD dma(wave, lane, xrb, a.D);
+  int kd_n = -1;
+  if (walk.s >= 0) {
+    if (DOC) kd_n = walk.s * 32 + (lane & 31) < a.Sk ? kdoc[walk.s * 32 + (lane & 31)] : -1;
+    dma.issue(xbase, xrb, walk.s * 32, hi, a.D, DOC && walk.neg ? kdoc : nullptr, smem);
+  }
+  const long long row = (long long)bh * a.Sq + ic;
+  u32x4 qf[G::KS], dof[G::KS];
+  float delta = 0.f;
+  {
+    const char* orow = (const char*)a.out + (((long long)b * a.Sq + ic) * a.H + head) * a.D * 2;
+    const char* drow = (const char*)a.dout + ((long long)b * a.do_sb + (long long)ic * a.do_ss + (long long)head * a.do_sh) * 2;
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ++ks) {
+      qf[ks] = gfrag<false>(qbase + (long long)ic * a.q_ss * 2, ks, h, a.D, live).v;
+      const SFrag<false> g = gfrag<false>(drow, ks, h, a.D, live);
+      dof[ks] = g.v;
+      delta += frag_dot<false>(g, gfrag<false>(orow, ks, h, a.D, live));
+    }
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  const float lse = live ? a.lse[row] : INFINITY;
+  f32x16 dq[G::DB];
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
+  float dsl = 0.f;
+  const SAddr<HDP> fk0(lds_addr_of(smem), lane);
+  int buf = 0;
+  while (walk.s >= 0) {
+    const int kv0 = walk.s * 32;
+    const bool full_t = walk.full && kv0 + 31 <= lim_lo, work = wave_live && kv0 <= lim_hi;
+    const int kd = kd_n;
+    walk.next(dsh, wave, lane);
+    dma_wait_barrier();                   // this pair is there; every wave is done with the one before
+    if (walk.s >= 0) {
+      if (DOC) kd_n = walk.s * 32 + (lane & 31) < a.Sk ? kdoc[walk.s * 32 + (lane & 31)] : -1;
+      dma.issue(xbase, xrb, walk.s * 32, hi, a.D, DOC && walk.neg ? kdoc : nullptr, smem + (buf ^ 1) * PD::BUF);
+    }
+    if (work) {
+      const SAddr<HDP> fk = shifted(fk0, buf * PD::BUF), fv = shifted(fk, PD::HALF);
+      f32x16 st, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = 0.f; }
+      pair_rows<HDP>(fk, fv, qf, dof, st, dp);
+      unsigned bits = 0xffffffffu;
+      if (!full_t) {
+        const int n = lim - kv0 + 1;
+        bits = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+        if (DOC) bits &= (unsigned)doc_bits(qd, kd);
+        bits >>= 4 * h;
+      }
+      const float pd = (float)(p - kv0 - 4 * h), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
+      unsigned pk[8];
+      by_flags(full_t, m.capl != 0.f, m.slope2 != 0.f || a.dslopes != nullptr, [&](auto FULL, auto CAP, auto SLP) {
+        auto one = [&](int r) {
+          const int j = (r & 3) + 8 * (r >> 2);
+          float t = CAP ? m.capl * tanh_of<false>(st[r] * m.sc) : st[r] * m.sc, x = t;
+          const float dist = SLP ? fabsf(pd - (float)j) : 0.f;
+          if (SLP) x -= m.slope2 * dist;
+          x = fast_exp2(x - lse) * (dp[r] - delta);
+          if (!FULL) x = (bits >> j) & 1u ? x : 0.f;
+          if (SLP) dsl -= x * dist;
+          return CAP ? x * fmaf(t * t, ncap, 1.0f) : x;           // the cap's derivative: 1 - (t / cap)^2
+        };
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float x0 = one(r), x1 = one(r + 1);
+          pk[r >> 1] = pk2(x0, x1);
+        }
+      });
+      tile_t<HDP>(fk, pk, dq);
+    }
+    buf ^= 1;
+  }
+  dsl += __shfl_xor(dsl, 32, 64);
+  if (i < a.Sq && h == 0) {
+    a.delta[row] = delta;
+    if (a.dslopes != nullptr) a.dslope_rows[row] = live ? dsl : 0.f;
+  }
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[d][r] = live ? dq[d][r] : 0.f;
+  store_lane_row<G::DB>((u16*)a.dq + (((long long)b * a.Sq + ic) * a.H + head) * a.D, dq, a.scale, h, a.D, i < a.Sq);
+}
+
+// dk, dv: key on the lane, 128 keys a workgroup.  PART 0: dv, 1: dk, 2: both
+template <int HDP, int PART, bool DOC>
+__global__ __launch_bounds__(256, (HDP <= (PART == 2 ? (DOC ? 64 : 96) : PART == 1 ? 128 : 192) ? 2 : 1)) void score_dkv16_kernel(const TfScoreAttnArgs a, int nkb) {
+  using G = SGeo<HDP>;
+  using PD = PairDma<HDP>;
+  constexpr bool DK = PART != 0, DV = PART != 1;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  float* stat = (float*)(smem + 2 * PD::BUF);             // [2 images][32 lse, 32 delta]
+  u64 (*dsh)[3] = (u64 (*)[3])(smem + 2 * PD::BUF + 512);
+  int* rsh = (int*)(smem + 2 * PD::BUF + 512 + 96);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int logical = xcd_remap(blockIdx.x, gridDim.x);
+  const int kb = logical % nkb, bk = logical / nkb, b = bk / a.Hk, kvh = bk % a.Hk, G_ = a.H / a.Hk;
+  const char* kbase = (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * 2;
+  const char* vbase = (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * 2;
+  const int* qdoc = DOC ? a.q_doc + (size_t)b * a.Sq : nullptr;
+  const int p0 = q_pos0(a, b), pfx = prefix_of(a, b);
+  const int k0 = kb * 128, w0 = k0 + wave * 32, j = w0 + (lane & 31), jc = min(j, a.Sk - 1);
+  const int kd = DOC ? a.k_doc[(size_t)b * a.Sk + jc] : 0;
+  const bool live = j < a.Sk && kd >= 0, wave_live = w0 < a.Sk;
+  u32x4 kf[G::KS], vf[DK ? G::KS : 1];
+#pragma unroll
+  for (int ks = 0; ks < G::KS; ++ks) {
+    kf[ks] = gfrag<false>(kbase + (long long)jc * a.k_ss * 2, ks, h, a.D, live).v;
+    if constexpr (DK) vf[ks] = gfrag<false>(vbase + (long long)jc * a.v_ss * 2, ks, h, a.D, live).v;
+  }
+  f32x16 dk[DK ? G::DB : 1], dv[DV ? G::DB : 1];
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if constexpr (DK) dk[d][r] = 0.f;
+      if constexpr (DV) dv[d][r] = 0.f;
+    }
+  // queries from q_lane on see this lane's key; the block's first key is seen from i_lo on, the wave's last key by all from q_full on
+  const int q_lane = a.causal && j >= pfx ? j - p0 : -(1 << 30);
+  const int i_lo = a.causal && k0 >= pfx ? min(max(k0 - p0, 0), a.Sq) : 0;
+  const int w_last = min(w0 + 31, a.Sk - 1);
+  const int q_full = a.causal && w_last >= pfx ? w_last - p0 : -(1 << 30), q_any = a.causal && w0 >= pfx ? w0 - p0 : -(1 << 30);
+  HalfWalk<DOC> walk{{qdoc, (a.Sq + 63) / 64, a.Sq, 0, 0, 0, {}, true, false}, -1, a.Sq, true, false};
+  if (DOC) {
+    const int lo = wave_min_i(live ? kd : 0x7fffffff), up = -wave_min_i(live ? -kd : 0x7fffffff);
+    if (lane == 0) { rsh[wave] = lo; rsh[4 + wave] = up; }
+    __syncthreads();
+    walk.w.dmin = __builtin_amdgcn_readfirstlane(min(min(rsh[0], rsh[1]), min(rsh[2], rsh[3])));
+    walk.w.dmax = __builtin_amdgcn_readfirstlane(max(max(rsh[4], rsh[5]), max(rsh[6], rsh[7])));
+  }
+  const unsigned xrb = (unsigned)(wave < 2 ? a.q_ss : a.do_ss) * 2;
+  const PD dma(wave, lane, xrb, a.D);
+  const SAddr<HDP> fq0(lds_addr_of(smem), lane);
+  const unsigned stat0 = lds_addr_of(stat) + 16 * h;
+  for (int g = 0; g < G_; ++g) {
+    const int head = kvh * G_ + g;
+    const SMod m = smod(a, head);
+    const char* xbase = wave < 2 ? (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * 2
+                                 : (const char*)a.dout + ((long long)b * a.do_sb + (long long)head * a.do_sh) * 2;
+    const long long row0 = ((long long)b * a.H + head) * a.Sq;
+    int qd_n = -1;
+    auto fetch = [&](int buf) {           // the pair in walk.s, its rows' statistics (wave 0: 32 of each, 4 bytes a lane) and documents
+      const int i0 = walk.s * 32;
+      if (DOC) qd_n = i0 + (lane & 31) < a.Sq ? qdoc[i0 + (lane & 31)] : -1;
+      dma.issue(xbase, xrb, i0, a.Sq, a.D, DOC && walk.neg ? qdoc : nullptr, smem + buf * PD::BUF);
+      if (wave == 0) {
+        const float* src = (lane < 32 ? a.lse : a.delta) + row0 + min(i0 + (lane & 31), a.Sq - 1);
+        __builtin_amdgcn_global_load_lds(TF_GLB_PTR(src), TF_LDS_PTR(stat + buf * 64), 4, 0, 0);
+      }
+    };
+    walk.first(i_lo / 32, dsh, wave, lane);
+    int buf = 0;
+    if (g > 0) __syncthreads();           // every wave is done with the images of the head before
+    if (walk.s >= 0) fetch(0);
+    while (walk.s >= 0) {
+      const int i0 = walk.s * 32;
+      const bool full_t = walk.full && i0 >= q_full && i0 + 32 <= a.Sq, work = wave_live && i0 + 31 >= q_any;
+      const int qd = qd_n;
+      walk.next(dsh, wave, lane);
+      dma_wait_barrier();
+      if (walk.s >= 0) fetch(buf ^ 1);
+      if (work) {
+        const SAddr<HDP> fq = shifted(fq0, buf * PD::BUF), fd = shifted(fq, PD::HALF);
+        f32x16 st, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = 0.f; }
+        if constexpr (DK) pair_rows<HDP>(fq, fd, kf, vf, st, dp);
+        else one_rows<HDP>(fq, kf, st);
+        u32x4 ls[4], de[4];               // register 4 g + e is query 8 g + 4 h + e
+        const unsigned sa = stat0 + buf * 256;
+        static_for<4>([&](auto I) { ls[I] = rd128_asm<32 * I>(sa); });
+        if constexpr (DK) static_for<4>([&](auto I) { de[I] = rd128_asm<128 + 32 * I>(sa); });
+        unsigned bits = 0xffffffffu;
+        if (!full_t) {
+          const int n = max(q_lane - i0, 0), e = a.Sq - i0;
+          bits = n >= 32 ? 0u : 0xffffffffu << n;
+          if (e < 32) bits &= (1u << e) - 1u;
+          if (DOC) bits &= (unsigned)doc_bits(kd, qd);
+          bits >>= 4 * h;
+        }
+        static_for<4>([&](auto I) { lgkm_wait<0>(ls[I]); });
+        if constexpr (DK) static_for<4>([&](auto I) { lgkm_wait<0>(de[I]); });
+        const float pd = (float)(p0 + i0 + 4 * h - j), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
+        unsigned pp[8], ps[8];
+        by_flags(full_t, m.capl != 0.f, m.slope2 != 0.f, [&](auto FULL, auto CAP, auto SLP) {
+          auto one = [&](int r, float& pr, float& ds) {
+            const int q = (r & 3) + 8 * (r >> 2);
+            float t = CAP ? m.capl * tanh_of<false>(st[r] * m.sc) : st[r] * m.sc, x = t;
+            if (SLP) x -= m.slope2 * fabsf(pd + (float)q);
+            pr = fast_exp2(x - f_of(ls[r >> 2][r & 3]));
+            if (!FULL) pr = (bits >> q) & 1u ? pr : 0.f;
+            if constexpr (DK) {
+              ds = pr * (dp[r] - f_of(de[r >> 2][r & 3]));
+              if (CAP) ds *= fmaf(t * t, ncap, 1.0f);
+              if (!FULL) ds = (bits >> q) & 1u ? ds : 0.f;        // (a hidden pair's product may not be finite)
+            }
+          };
+#pragma unroll
+          for (int r = 0; r < 16; r += 2) {
+            float p0_, p1_, s0_ = 0.f, s1_ = 0.f;
+            one(r, p0_, s0_);
+            one(r + 1, p1_, s1_);
+            if constexpr (DV) pp[r >> 1] = pk2(p0_, p1_);
+            if constexpr (DK) ps[r >> 1] = pk2(s0_, s1_);
+          }
+        });
+        if constexpr (DV) tile_t<HDP>(fd, pp, dv);
+        if constexpr (DK) tile_t<HDP>(fq, ps, dk);
+      }
+      buf ^= 1;
+    }
+  }
+  const long long go = (((long long)b * a.Sk + jc) * a.Hk + kvh) * a.D;
+  if constexpr (DK) {
+#pragma unroll
+    for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dk[d][r] = live ? dk[d][r] : 0.f;
+    store_lane_row<G::DB>((u16*)a.dk + go, dk, a.scale, h, a.D, j < a.Sk);
+  }
+  if constexpr (DV) {
+#pragma unroll
+    for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dv[d][r] = live ? dv[d][r] : 0.f;
+    store_lane_row<G::DB>((u16*)a.dv + go, dv, 1.0f, h, a.D, j < a.Sk);
+  }
+}
+
+// ================================================================================================
 // launchers
 // ================================================================================================
 // dynamic LDS beyond the default limit is granted per device
@@ -928,24 +1327,32 @@ template <bool F32, int HDP> int launch_fwd(const TfScoreAttnArgs* a, hipStream_
 template <bool F32, int HDP> int launch_bwd(const TfScoreAttnArgs* a, hipStream_t st) {
   const double fl = 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D;
   const int nqb = (a->Sq + 127) / 128, nkb = (a->Sk + 127) / 128;
-  const size_t lds = 64 * STile<F32, HDP>::STR + 32 * 16;
+  const bool doc = a->k_doc != nullptr;
+  const size_t lds = F32 ? 64 * STile<true, HDP>::STR + 32 * 16 : 2 * PairDma<HDP>::BUF + 512 + 128;
+  auto go = [&](auto kern, int blocks, int n) {
+    allow_lds(kern, lds);
+    hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), lds, st, *a, n);
+  };
   if (nqb > 0) {
-    allow_lds(score_dq_kernel<F32, HDP>, lds);
-    TfTraceScope tr(F32 ? "score_dq_kernel<fp32>" : "score_dq_kernel<bf16>", st, 1.5 * fl);
-    hipLaunchKernelGGL((score_dq_kernel<F32, HDP>), dim3(a->B * a->H * nqb), dim3(256), lds, st, *a, nqb);
+    TfTraceScope tr(F32 ? "score_dq_kernel" : "score_dq16_kernel", st, 1.5 * fl);
+    const int blocks = a->B * a->H * nqb;
+    if constexpr (F32) go(score_dq_kernel<true, HDP>, blocks, nqb);
+    else doc ? go(score_dq16_kernel<HDP, true>, blocks, nqb) : go(score_dq16_kernel<HDP, false>, blocks, nqb);
   }
   if (a->dslopes != nullptr) {
     TfTraceScope tr("score_dslope_kernel", st);
     hipLaunchKernelGGL(score_dslope_kernel, dim3(a->H), dim3(256), 0, st, (const float*)a->dslope_rows, a->dslopes, a->B, a->H, a->Sq);
   }
   if (nkb > 0) {
-    TfTraceScope tr(F32 ? "score_dkv_kernel<fp32>" : "score_dkv_kernel<bf16>", st, 2.0 * fl);
-    auto go = [&](auto kern) {
-      allow_lds(kern, lds);
-      hipLaunchKernelGGL(kern, dim3(a->B * a->Hk * nkb), dim3(256), lds, st, *a, nkb);
+    TfTraceScope tr(F32 ? "score_dkv_kernel" : "score_dkv16_kernel", st, 2.0 * fl);
+    const int blocks = a->B * a->Hk * nkb;
+    auto part = [&](auto which) {
+      constexpr int PART = decltype(which)::value;
+      if constexpr (F32) go(score_dkv_kernel<true, HDP, PART>, blocks, nkb);
+      else doc ? go(score_dkv16_kernel<HDP, PART, true>, blocks, nkb) : go(score_dkv16_kernel<HDP, PART, false>, blocks, nkb);
     };
-    if constexpr (HDP <= (F32 ? 128 : 192)) go(score_dkv_kernel<F32, HDP, 2>);
-    else { go(score_dkv_kernel<F32, HDP, 0>); go(score_dkv_kernel<F32, HDP, 1>); }
+    if constexpr (HDP <= (F32 ? 128 : 192)) part(std::integral_constant<int, 2>{});
+    else { part(std::integral_constant<int, 0>{}); part(std::integral_constant<int, 1>{}); }
   }
   return (int)hipGetLastError();
 }
