@@ -138,6 +138,14 @@ CASES = {
     "far slopes": (1, 64, 1100, 2, 2, 64, {"causal": 1, "slopes": 30}),  # steep: far keys vanish
     "long split": (1, 3, 1500, 8, 2, 64, {"causal": 1, "cap": 10.0}),
     "group rows": (2, 7, 513, 14, 2, 64, {"causal": 1, "slopes": 1, "pad": 1}),
+    "token documents": (3, 1, 700, 6, 2, 40, {"docs": -3, "slopes": 1}),
+    "token behind padding": (3, 2, 900, 8, 1, 192, {"causal": 1, "pad": 1, "cap": 6.0}),
+    "token wide": (2, 1, 333, 4, 4, 256, {"causal": 1, "slopes": 1}),
+    "token wide padding": (2, 3, 260, 4, 2, 256, {"causal": 1, "pad": 1}),
+    "token caches": (4, 1, 1000, 8, 2, 96, {"causal": 1, "start": 1, "prefix": 1}),
+    "32 rows": (2, 4, 222, 8, 1, 128, {"causal": 1}),
+    "33 rows": (2, 33, 222, 1, 1, 32, {"causal": 1}),
+    "few rows split": (1, 40, 2100, 2, 1, 64, {"causal": 1, "slopes": 1, "pad": 1}),
 }
 
 

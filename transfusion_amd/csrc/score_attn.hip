@@ -613,6 +613,368 @@ __global__ __launch_bounds__(256, (HDP <= 192 ? 2 : 1)) void score_fwd16_kernel(
   if (i < a.Sq && h == 0 && a.lse != nullptr) a.lse[row] = none ? INFINITY : m_run + log2f(l_tot);
 }
 
+// Two 32-row tiles that are used together (K and V, or Q and dO), staged as one image of 64 rows: waves 0 and 1 fetch the first matrix,
+// 2 and 3 the second.  Two images: the next pair travels under the whole of this one's work, one barrier a pair.
+template <int HDP> struct PairDma {
+  static constexpr int T = SGeo<HDP>::STR, NI = 64 * T / 4096, HALF = 32 * T, BUF = 64 * T;
+  unsigned off[NI];
+  int wave, lane;
+  __device__ __forceinline__ int row(int i) const { return ((wave & 1) * NI * 1024 + i * 1024 + lane * 16) / T; }
+  __device__ __forceinline__ PairDma(int wave_, int lane_, unsigned row_bytes, int D) : wave(wave_), lane(lane_) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int pos = (wave & 1) * NI * 1024 + i * 1024 + lane * 16, r = pos / T, cp = (pos % T) >> 4, c = cp ^ ((r >> 2) & 3);
+      off[i] = cp >= HDP / 8 || c * 8 >= D ? SDma<HDP>::OUT : (unsigned)r * row_bytes + c * 16;
+    }
+  }
+  // base, row_bytes: of the matrix this wave fetches.  Rows at or beyond row_end and (doc != null) rows of negative documents: zeros
+  __device__ __forceinline__ void issue(const char* base, unsigned row_bytes, int row0, int row_end, int D, const int* doc, unsigned char* image) const {
+    const int n = min(32, row_end - row0);
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(base + (long long)row0 * row_bytes), 0, (int)((unsigned)(n - 1) * row_bytes + D * 2), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      unsigned o = off[i];
+      if (doc != nullptr && doc[row0 + min(row(i), n - 1)] < 0) o = SDma<HDP>::OUT;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TF_LDS_PTR(image + (wave * NI + i) * 1024), 16, (int)o, 0, 0, 0);
+    }
+  }
+};
+// st += X . x and dp += Y . y of a pair image: row fragments PF ahead of their matrix instruction, the two accumulators in turn
+template <int HDP> __device__ __forceinline__ void pair_rows(const SAddr<HDP>& fx, const SAddr<HDP>& fy, const u32x4 (&x)[HDP / 16], const u32x4 (&y)[HDP / 16],
+                                                             f32x16& st, f32x16& dp) {
+  constexpr int NF = 2 * (HDP / 16), PF = 4;
+  u32x4 fr[NF];
+  static_for<PF>([&](auto I) { if constexpr (I & 1) fr[I] = fy.template row<0, (I >> 1)>(); else fr[I] = fx.template row<0, (I >> 1)>(); });
+  static_for<NF>([&](auto I) {
+    constexpr int i = I, nx = i + PF;
+    if constexpr (nx < NF) { if constexpr (nx & 1) fr[nx] = fy.template row<0, (nx >> 1)>(); else fr[nx] = fx.template row<0, (nx >> 1)>(); }
+    lgkm_wait<(NF - 1 - i < PF ? NF - 1 - i : PF)>(fr[i]);
+    if constexpr (i & 1) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(fr[i]), as_bf16x8(y[i >> 1]), dp, 0, 0, 0);
+    else st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(fr[i]), as_bf16x8(x[i >> 1]), st, 0, 0, 0);
+  });
+}
+template <int HDP> __device__ __forceinline__ void one_rows(const SAddr<HDP>& fx, const u32x4 (&x)[HDP / 16], f32x16& st) {
+  constexpr int NF = HDP / 16, PF = NF < 4 ? NF : 4;
+  u32x4 fr[NF];
+  static_for<PF>([&](auto I) { fr[I] = fx.template row<0, I>(); });
+  static_for<NF>([&](auto I) {
+    constexpr int i = I, nx = i + PF;
+    if constexpr (nx < NF) fr[nx] = fx.template row<0, nx>();
+    lgkm_wait<(NF - 1 - i < PF ? NF - 1 - i : PF)>(fr[i]);
+    st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(fr[i]), as_bf16x8(x[i]), st, 0, 0, 0);
+  });
+}
+// acc[channel][lane] += sum over the 32 rows of a tile of tile[row][channel] * p[row]; p: 16 values packed as they lie in the accumulator
+template <int HDP> __device__ __forceinline__ void tile_t(const SAddr<HDP>& f, const unsigned (&p)[8], f32x16 (&acc)[HDP / 32]) {
+  constexpr int DB = HDP / 32, NF = 2 * DB, PF = 2;
+  u64 fa[NF], fb[NF];
+  static_for<PF>([&](auto I) { f.template tr<(I / DB) * 16, (I % DB) * 32>(fa[I], fb[I]); });
+  static_for<NF>([&](auto I) {
+    constexpr int i = I, nx = i + PF, s = 4 * (i / DB);
+    if constexpr (nx < NF) f.template tr<(nx / DB) * 16, (nx % DB) * 32>(fa[nx], fb[nx]);
+    lgkm_wait<2 * (NF - 1 - i < PF ? NF - 1 - i : PF)>(fa[i], fb[i]);
+    acc[i % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join_tr64(fa[i], fb[i]), as_bf16x8(u32x4{p[s], p[s + 1], p[s + 2], p[s + 3]}), acc[i % DB], 0, 0, 0);
+  });
+}
+template <int HDP> __device__ __forceinline__ SAddr<HDP> shifted(const SAddr<HDP>& f, unsigned bytes) {
+  SAddr<HDP> g = f;
+  g.row_e += bytes; g.row_o += bytes; g.tr_a += bytes; g.tr_b += bytes;
+  return g;
+}
+
+// ================================================================================================
+// forward of few rows (single tokens): Sq * H / Hk <= 32
+// ================================================================================================
+// Bound by the bytes of K and V.  The rows of all heads that share a key head are one 32-column tile, so every key is read once; each of
+// the four waves walks key tiles of its own (32 keys) and the workgroup's keys are a range of the sample's (the launcher splits the keys
+// until the chip is full).  bf16: no barrier in the loop -- a wave waits for its own transfers by count: K(t + 1) is under way from the
+// moment S(t) has been read, V(t + 1) from the end of PV(t), so one tile is always in flight.  The waves' parts are joined in LDS.
+struct FewRows { int i, head, lim, qd; bool ok, live; float slope2; };
+__device__ __forceinline__ FewRows few_rows(const TfScoreAttnArgs& a, int b, int kvh, int p0, int pfx, int lane) {
+  FewRows w;
+  const int G = a.H / a.Hk, r = lane & 31;
+  w.ok = r < a.Sq * G;
+  const int rc = w.ok ? r : 0;
+  w.i = rc / G;
+  w.head = kvh * G + rc % G;
+  w.qd = a.k_doc != nullptr ? a.q_doc[(size_t)b * a.Sq + w.i] : 0;
+  w.live = w.ok && w.qd >= 0;
+  w.lim = a.causal ? min(max(p0 + w.i, pfx - 1), a.Sk - 1) : a.Sk - 1;
+  w.slope2 = a.slopes != nullptr ? a.slopes[w.head] * LOG2E : 0.f;
+  return w;
+}
+// the changed and masked scores of a 32-key tile (kd: document of key kv0 + (lane & 31))
+template <bool F32, bool DOC> __device__ __forceinline__ void few_change(const TfScoreAttnArgs& a, const FewRows& w, const SMod& m, int p0, int kv0, int kd, int h,
+                                                                         f32x16& st) {
+  if (m.capl != 0.f) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st[r] = m.capl * tanh_of<F32>(st[r] * m.sc);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st[r] *= m.sc;
+  }
+  if (a.slopes != nullptr) {
+    const float pd = (float)(p0 + w.i - kv0 - 4 * h);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st[r] -= w.slope2 * fabsf(pd - (float)((r & 3) + 8 * (r >> 2)));
+  }
+  const int n = w.lim - kv0 + 1;
+  unsigned bits = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+  if (DOC) bits &= (unsigned)doc_bits(w.qd, kd);
+  if (__any(bits != 0xffffffffu)) {
+    bits >>= 4 * h;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (!((bits >> ((r & 3) + 8 * (r >> 2))) & 1u)) st[r] = -INFINITY;
+  }
+}
+// one step of the running softmax over a 32-key tile: st becomes the probabilities
+template <int DB> __device__ __forceinline__ void few_softmax(f32x16& st, float& m_run, float& l_run, f32x16 (&o)[DB]) {
+  float mx = -INFINITY;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[r]);
+  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+  const bool need = mx - m_run > RESCALE_THR;
+  if (__any(need)) {
+    const float m_new = need ? fmaxf(m_run, mx) : m_run, alpha = need ? fast_exp2(m_run - m_new) : 1.0f;
+    m_run = m_new;
+    l_run *= alpha;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    st[r] = fast_exp2(st[r] - m_run);
+    l_run += st[r];
+  }
+}
+// joins the four waves' parts (smem: 4 * 32 * D + 256 floats) and writes the rows, or this split's part of them
+template <bool F32, int DB> __device__ __forceinline__ void few_finish(const TfScoreAttnArgs& a, const FewRows& w, int b, int kvh, float m_run, float l_run,
+                                                                       f32x16 (&o)[DB], float* smem, int nsplit, int split, int wave, int lane) {
+  const int h = lane >> 5, r = lane & 31, G = a.H / a.Hk, R = a.Sq * G;
+  float* ml = smem + 128 * a.D;                          // [4 waves][32][2]
+  const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+  const bool none = !w.live || l_tot == 0.f;
+  __syncthreads();
+  if (h == 0) { ml[(wave * 32 + r) * 2] = none ? S_NEG : m_run; ml[(wave * 32 + r) * 2 + 1] = none ? 0.f : l_tot; }
+  __syncthreads();
+  float mx = S_NEG;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) mx = fmaxf(mx, ml[(v * 32 + r) * 2]);
+  const float s = none ? 0.f : fast_exp2(m_run - mx);
+  if (w.ok) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = d * 32 + 8 * g + 4 * h;
+        if (c < a.D) *(f32x4*)(smem + (wave * 32 + r) * a.D + c) = none ? f32x4{0, 0, 0, 0} : f32x4{o[d][4 * g] * s, o[d][4 * g + 1] * s, o[d][4 * g + 2] * s, o[d][4 * g + 3] * s};
+      }
+  }
+  __syncthreads();
+  const int d4 = a.D / 4;
+  const long long rows = (long long)a.B * a.H * a.Sq;
+  for (int x = wave * 64 + lane; x < R * d4; x += 256) {
+    const int q = x / d4, c = x % d4 * 4, i = q / G, head = kvh * G + q % G;
+    float top = S_NEG, l = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) top = fmaxf(top, ml[(v * 32 + q) * 2]);
+    f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      l += ml[(v * 32 + q) * 2 + 1] * fast_exp2(ml[(v * 32 + q) * 2] - top);
+      acc += *(const f32x4*)(smem + (v * 32 + q) * a.D + c);
+    }
+    const long long row = ((long long)b * a.H + head) * a.Sq + i;
+    if (nsplit > 1) {
+      *(f32x4*)((float*)a.work + ((long long)split * rows + row) * a.D + c) = acc;
+      if (c == 0) {
+        float* pml = (float*)a.work + (long long)nsplit * rows * a.D + ((long long)split * rows + row) * 2;
+        pml[0] = top;
+        pml[1] = l;
+      }
+    } else {
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      const long long oo = (((long long)b * a.Sq + i) * a.H + head) * a.D + c;
+      if constexpr (F32) *(f32x4*)((float*)a.out + oo) = acc * inv;
+      else *(u32x2*)((u16*)a.out + oo) = u32x2{pk2(acc[0] * inv, acc[1] * inv), pk2(acc[2] * inv, acc[3] * inv)};
+      if (c == 0 && a.lse != nullptr) a.lse[row] = l == 0.f ? INFINITY : top + log2f(l);
+    }
+  }
+}
+// keys of a workgroup: an equal share of the tiles this sample's rows can see
+struct FewRange { int lo, end, hi; };
+__device__ __forceinline__ FewRange few_range(const TfScoreAttnArgs& a, int p0, int pfx, int nsplit, int split) {
+  FewRange f;
+  f.hi = a.causal ? max(0, min(max(p0 + a.Sq, pfx), a.Sk)) : a.Sk;
+  const int tiles = (f.hi + 31) / 32;
+  f.lo = (int)((long long)tiles * split / nsplit);
+  f.end = (int)((long long)tiles * (split + 1) / nsplit);
+  return f;
+}
+
+template <int N> __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+template <int HDP, bool DOC>
+__global__ __launch_bounds__(256, (HDP <= 128 ? 2 : 1)) void score_few16_kernel(const TfScoreAttnArgs a, int nsplit) {
+  using G = SGeo<HDP>;
+  constexpr int T = G::STR, NI = 32 * T / 1024;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  unsigned char* kt = smem + wave * 64 * T;
+  unsigned char* vt = kt + 32 * T;
+  const int logical = xcd_remap(blockIdx.x, gridDim.x), split = logical % nsplit, bk = logical / nsplit, b = bk / a.Hk, kvh = bk % a.Hk;
+  const char* kbase = (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * 2;
+  const char* vbase = (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * 2;
+  const unsigned krb = (unsigned)a.k_ss * 2, vrb = (unsigned)a.v_ss * 2;
+  const int* kdoc = DOC ? a.k_doc + (size_t)b * a.Sk : nullptr;
+  const int p0 = q_pos0(a, b), pfx = prefix_of(a, b);
+  const FewRows w = few_rows(a, b, kvh, p0, pfx, lane);
+  SMod m = smod(a, kvh * (a.H / a.Hk));
+  const FewRange f = few_range(a, p0, pfx, nsplit, split);
+  unsigned koff[NI], voff[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int pos = i * 1024 + lane * 16, r = pos / T, cp = (pos % T) >> 4, c = cp ^ ((r >> 2) & 3);
+    const bool out = cp >= HDP / 8 || c * 8 >= a.D;
+    koff[i] = out ? SDma<HDP>::OUT : (unsigned)r * krb + c * 16;
+    voff[i] = out ? SDma<HDP>::OUT : (unsigned)r * vrb + c * 16;
+  }
+  auto issue = [&](const char* base, unsigned rb, const unsigned (&off)[NI], int t, unsigned char* tile, bool neg) {
+    const int n = min(32, f.hi - t * 32);
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(base + (long long)t * 32 * rb), 0, (int)((unsigned)(n - 1) * rb + a.D * 2), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      unsigned x = off[i];
+      if (DOC && neg && kdoc[t * 32 + min((i * 1024 + lane * 16) / T, n - 1)] < 0) x = SDma<HDP>::OUT;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TF_LDS_PTR(tile + i * 1024), 16, (int)x, 0, 0, 0);
+    }
+  };
+  // documents: the tile's ids are read a tile ahead of its transfer; tiles without one of the rows' documents are passed over
+  const int dmin = DOC ? wave_min_i(w.live ? w.qd : 0x7fffffff) : 0, dmax = DOC ? -wave_min_i(w.live ? -w.qd : 0x7fffffff) : 0;
+  auto doc_of = [&](int t) { const int j = t * 32 + (lane & 31); return j < a.Sk ? kdoc[j] : -1; };
+  bool neg = false;
+  int kd = 0, kd_n = 0, kd_nn = 0;                       // of the tile in hand, the tile under way, the tile after it
+  auto seek = [&](int t) {                               // first visible tile from t on; leaves its documents in kd_n
+    if (!DOC) return t < f.end ? t : -1;
+    for (; t < f.end; t += 4) {
+      kd_n = kd_nn;
+      if (t + 4 < f.end) kd_nn = doc_of(t + 4);
+      if (__any(kd_n >= dmin && kd_n <= dmax)) { neg = __any(kd_n < 0); return t; }
+    }
+    return -1;
+  };
+  u32x4 qf[G::KS];
+  {
+    const char* qrow = (const char*)a.q + ((long long)b * a.q_sb + (long long)w.i * a.q_ss + (long long)w.head * a.q_sh) * 2;
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ++ks) qf[ks] = gfrag<false>(qrow, ks, h, a.D, w.live).v;
+  }
+  f32x16 o[G::DB];
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m_run = S_NEG, l_run = 0.f;
+  const SAddr<HDP> fk(lds_addr_of(kt), lane), fv(lds_addr_of(vt), lane);
+  if (DOC && f.lo + wave < f.end) kd_nn = doc_of(f.lo + wave);
+  int t = seek(f.lo + wave);
+  bool neg_t = neg;
+  if (t >= 0) {
+    kd = kd_n;
+    issue(kbase, krb, koff, t, kt, neg);
+    issue(vbase, vrb, voff, t, vt, neg);
+  }
+  while (t >= 0) {
+    const int tn = seek(t + 4), kd_next = kd_n;
+    neg_t = neg;
+    vm_wait<NI>();                        // K(t); V(t)'s NI transfers may still be out
+    f32x16 st;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st[r] = 0.f;
+    one_rows<HDP>(fk, qf, st);
+    if (tn >= 0) issue(kbase, krb, koff, tn, kt, neg_t);
+    few_change<false, DOC>(a, w, m, p0, t * 32, kd, h, st);
+    few_softmax<G::DB>(st, m_run, l_run, o);
+    unsigned pk[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) pk[r] = pk2(st[2 * r], st[2 * r + 1]);
+    if (tn >= 0) vm_wait<NI>(); else vm_wait<0>();       // V(t); K(t + 1)'s may still be out
+    tile_t<HDP>(fv, pk, o);
+    if (tn >= 0) issue(vbase, vrb, voff, tn, vt, neg_t);
+    kd = kd_next;
+    t = tn;
+  }
+  few_finish<false, G::DB>(a, w, b, kvh, m_run, l_run, o, (float*)smem, nsplit, split, wave, lane);
+}
+
+// fp32: K fragments and V rows come straight from memory (V's are whole 128-byte lines a half-wave, the fp32 matrix instruction takes them
+// untransposed), so nothing is staged; many waves hide the latency
+template <int HDP, bool DOC>
+__global__ __launch_bounds__(256, 1) void score_few32_kernel(const TfScoreAttnArgs a, int nsplit) {
+  constexpr int KS = HDP / 16, DB = HDP / 32;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int logical = xcd_remap(blockIdx.x, gridDim.x), split = logical % nsplit, bk = logical / nsplit, b = bk / a.Hk, kvh = bk % a.Hk;
+  const char* kbase = (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * 4;
+  const char* vbase = (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * 4;
+  const int* kdoc = DOC ? a.k_doc + (size_t)b * a.Sk : nullptr;
+  const int p0 = q_pos0(a, b), pfx = prefix_of(a, b);
+  const FewRows w = few_rows(a, b, kvh, p0, pfx, lane);
+  const SMod m = smod(a, kvh * (a.H / a.Hk));
+  const FewRange f = few_range(a, p0, pfx, nsplit, split);
+  const int dmin = DOC ? wave_min_i(w.live ? w.qd : 0x7fffffff) : 0, dmax = DOC ? -wave_min_i(w.live ? -w.qd : 0x7fffffff) : 0;
+  constexpr bool REREAD = HDP > 192;      // Q does not fit beside the accumulators: read again (from L1) for every tile
+  const char* qrow = (const char*)a.q + ((long long)b * a.q_sb + (long long)w.i * a.q_ss + (long long)w.head * a.q_sh) * 4;
+  SFrag<true> qf[REREAD ? 1 : KS];
+  if constexpr (!REREAD) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = gfrag<true>(qrow, ks, h, a.D, w.live);
+  }
+  f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+  float m_run = S_NEG, l_run = 0.f;
+  for (int t = f.lo + wave; t < f.end; t += 4) {
+    const int kv0 = t * 32, j = kv0 + (lane & 31);
+    int kd = 0;
+    if (DOC) {
+      kd = j < a.Sk ? kdoc[j] : -1;
+      if (!__any(kd >= dmin && kd <= dmax)) continue;
+    }
+    f32x16 st;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st[r] = 0.f;
+    const char* krow = kbase + (long long)min(j, f.hi - 1) * a.k_ss * 4;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const SFrag<true> x = gfrag<true>(krow, ks, h, a.D, j < f.hi && (!DOC || kd >= 0));
+      if constexpr (REREAD) st = smma<true>(x, gfrag<true>(qrow, ks, h, a.D, w.live), st);
+      else st = smma<true>(x, qf[ks], st);
+    }
+    few_change<true, DOC>(a, w, m, p0, kv0, kd, h, st);
+    few_softmax<DB>(st, m_run, l_run, o);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int jj = (r & 3) + 8 * (r >> 2) + 4 * h;
+      const bool in = kv0 + jj < f.hi && (!DOC || __shfl(kd, jj, 64) >= 0);
+      const float* vrow = (const float*)(vbase + (long long)min(kv0 + jj, f.hi - 1) * a.v_ss * 4) + (lane & 31);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const float v = in && d * 32 + (lane & 31) < a.D ? vrow[d * 32] : 0.f;
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, st[r], o[d], 0, 0, 0);
+      }
+    }
+  }
+  few_finish<true, DB>(a, w, b, kvh, m_run, l_run, o, (float*)smem, nsplit, split, wave, lane);
+}
+
 // joins the parts of a split forward: one wave a row, four channels a lane
 template <bool F32> __global__ __launch_bounds__(256) void score_join_kernel(const TfScoreAttnArgs a, int nsplit) {
   const long long rows = (long long)a.B * a.H * a.Sq, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -875,76 +1237,6 @@ __global__ __launch_bounds__(256, 1) void score_dkv_kernel(const TfScoreAttnArgs
 // ================================================================================================
 // backward, bf16
 // ================================================================================================
-// Two 32-row tiles that are used together (K and V, or Q and dO), staged as one image of 64 rows: waves 0 and 1 fetch the first matrix,
-// 2 and 3 the second.  Two images: the next pair travels under the whole of this one's work, one barrier a pair.
-template <int HDP> struct PairDma {
-  static constexpr int T = SGeo<HDP>::STR, NI = 64 * T / 4096, HALF = 32 * T, BUF = 64 * T;
-  unsigned off[NI];
-  int wave, lane;
-  __device__ __forceinline__ int row(int i) const { return ((wave & 1) * NI * 1024 + i * 1024 + lane * 16) / T; }
-  __device__ __forceinline__ PairDma(int wave_, int lane_, unsigned row_bytes, int D) : wave(wave_), lane(lane_) {
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int pos = (wave & 1) * NI * 1024 + i * 1024 + lane * 16, r = pos / T, cp = (pos % T) >> 4, c = cp ^ ((r >> 2) & 3);
-      off[i] = cp >= HDP / 8 || c * 8 >= D ? SDma<HDP>::OUT : (unsigned)r * row_bytes + c * 16;
-    }
-  }
-  // base, row_bytes: of the matrix this wave fetches.  Rows at or beyond row_end and (doc != null) rows of negative documents: zeros
-  __device__ __forceinline__ void issue(const char* base, unsigned row_bytes, int row0, int row_end, int D, const int* doc, unsigned char* image) const {
-    const int n = min(32, row_end - row0);
-    const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc((void*)(base + (long long)row0 * row_bytes), 0, (int)((unsigned)(n - 1) * row_bytes + D * 2), 0x00020000);
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      unsigned o = off[i];
-      if (doc != nullptr && doc[row0 + min(row(i), n - 1)] < 0) o = SDma<HDP>::OUT;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TF_LDS_PTR(image + (wave * NI + i) * 1024), 16, (int)o, 0, 0, 0);
-    }
-  }
-};
-// st += X . x and dp += Y . y of a pair image: row fragments PF ahead of their matrix instruction, the two accumulators in turn
-template <int HDP> __device__ __forceinline__ void pair_rows(const SAddr<HDP>& fx, const SAddr<HDP>& fy, const u32x4 (&x)[HDP / 16], const u32x4 (&y)[HDP / 16],
-                                                             f32x16& st, f32x16& dp) {
-  constexpr int NF = 2 * (HDP / 16), PF = 4;
-  u32x4 fr[NF];
-  static_for<PF>([&](auto I) { if constexpr (I & 1) fr[I] = fy.template row<0, (I >> 1)>(); else fr[I] = fx.template row<0, (I >> 1)>(); });
-  static_for<NF>([&](auto I) {
-    constexpr int i = I, nx = i + PF;
-    if constexpr (nx < NF) { if constexpr (nx & 1) fr[nx] = fy.template row<0, (nx >> 1)>(); else fr[nx] = fx.template row<0, (nx >> 1)>(); }
-    lgkm_wait<(NF - 1 - i < PF ? NF - 1 - i : PF)>(fr[i]);
-    if constexpr (i & 1) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(fr[i]), as_bf16x8(y[i >> 1]), dp, 0, 0, 0);
-    else st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(fr[i]), as_bf16x8(x[i >> 1]), st, 0, 0, 0);
-  });
-}
-template <int HDP> __device__ __forceinline__ void one_rows(const SAddr<HDP>& fx, const u32x4 (&x)[HDP / 16], f32x16& st) {
-  constexpr int NF = HDP / 16, PF = NF < 4 ? NF : 4;
-  u32x4 fr[NF];
-  static_for<PF>([&](auto I) { fr[I] = fx.template row<0, I>(); });
-  static_for<NF>([&](auto I) {
-    constexpr int i = I, nx = i + PF;
-    if constexpr (nx < NF) fr[nx] = fx.template row<0, nx>();
-    lgkm_wait<(NF - 1 - i < PF ? NF - 1 - i : PF)>(fr[i]);
-    st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(fr[i]), as_bf16x8(x[i]), st, 0, 0, 0);
-  });
-}
-// acc[channel][lane] += sum over the 32 rows of a tile of tile[row][channel] * p[row]; p: 16 values packed as they lie in the accumulator
-template <int HDP> __device__ __forceinline__ void tile_t(const SAddr<HDP>& f, const unsigned (&p)[8], f32x16 (&acc)[HDP / 32]) {
-  constexpr int DB = HDP / 32, NF = 2 * DB, PF = 2;
-  u64 fa[NF], fb[NF];
-  static_for<PF>([&](auto I) { f.template tr<(I / DB) * 16, (I % DB) * 32>(fa[I], fb[I]); });
-  static_for<NF>([&](auto I) {
-    constexpr int i = I, nx = i + PF, s = 4 * (i / DB);
-    if constexpr (nx < NF) f.template tr<(nx / DB) * 16, (nx % DB) * 32>(fa[nx], fb[nx]);
-    lgkm_wait<2 * (NF - 1 - i < PF ? NF - 1 - i : PF)>(fa[i], fb[i]);
-    acc[i % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(join_tr64(fa[i], fb[i]), as_bf16x8(u32x4{p[s], p[s + 1], p[s + 2], p[s + 3]}), acc[i % DB], 0, 0, 0);
-  });
-}
-template <int HDP> __device__ __forceinline__ SAddr<HDP> shifted(const SAddr<HDP>& f, unsigned bytes) {
-  SAddr<HDP> g = f;
-  g.row_e += bytes; g.row_o += bytes; g.tr_a += bytes; g.tr_b += bytes;
-  return g;
-}
-
 // [rows of a 32-row accumulator tile][channels] of one lane -> 16-byte stores (see the forward's epilogue)
 template <int DB> __device__ __forceinline__ void store_lane_row(u16* row, const f32x16 (&x)[DB], float scale, int h, int D, bool ok) {
 #pragma unroll
@@ -1277,9 +1569,16 @@ template <class K> void allow_lds(K kern, size_t bytes) {
 
 int hdp_of(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : D <= 192 ? 192 : 256; }
 
-struct FwdPlan { int nqb, nsplit, split_tiles; };
+struct FwdPlan { bool few; int nqb, nsplit, split_tiles; };
 FwdPlan fwd_plan(const TfScoreAttnArgs* a) {
   FwdPlan f;
+  f.few = (long long)a->Sq * (a->H / a->Hk) <= 32;
+  if (f.few) {                            // two workgroups a CU, each with at least two tiles a wave
+    const long long groups = (long long)a->B * a->Hk, tiles = (a->Sk + 31) / 32;
+    f.nqb = f.split_tiles = 0;
+    f.nsplit = (int)std::max(1ll, std::min((512 + groups - 1) / groups, tiles / 8));
+    return f;
+  }
   const int kt = a->is_f32 ? 32 : 64;
   f.nqb = (a->Sq + 127) / 128;
   const long long blocks = (long long)a->B * a->H * f.nqb;
@@ -1307,7 +1606,16 @@ bool aligned(const void* p, long long sb, long long ss, long long sh, int e) {
 
 template <bool F32, int HDP> int launch_fwd(const TfScoreAttnArgs* a, hipStream_t st) {
   const FwdPlan f = fwd_plan(a);
-  {
+  if (f.few) {
+    TfTraceScope tr(F32 ? "score_few32_kernel" : "score_few16_kernel", st, 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D);
+    const size_t join = (128 * (size_t)a->D + 256) * 4;
+    auto go = [&](auto kern, size_t lds) {
+      allow_lds(kern, std::max(lds, (size_t)(128 * HDP + 256) * 4));
+      hipLaunchKernelGGL(kern, dim3(a->B * a->Hk * f.nsplit), dim3(256), std::max(lds, join), st, *a, f.nsplit);
+    };
+    if constexpr (F32) a->k_doc != nullptr ? go(score_few32_kernel<HDP, true>, 0) : go(score_few32_kernel<HDP, false>, 0);
+    else a->k_doc != nullptr ? go(score_few16_kernel<HDP, true>, 256 * SGeo<HDP>::STR) : go(score_few16_kernel<HDP, false>, 256 * SGeo<HDP>::STR);
+  } else {
     TfTraceScope tr(F32 ? "score_fwd_kernel" : "score_fwd16_kernel", st, 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D);
     auto go = [&](auto kern, size_t lds) {
       allow_lds(kern, lds);
