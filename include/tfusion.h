@@ -628,14 +628,14 @@ typedef struct TfScoreAttnArgs {
   const float* slopes;                           // [H] fp32 or null
   int causal; const int* prefix; const int* q_start;   // [B] int32 device arrays or null
   const int* q_doc; const int* k_doc;            // [B, Sq] / [B, Sk] int32 contiguous, both or neither
-  void* work; size_t work_bytes;                 // forward: tf_score_attn_work(a) bytes (0: none needed)
+  void* work; size_t work_bytes;                 // forward: tf_score_attn_work(sizes) bytes (0: none needed)
   // backward (lse from the forward)
   const void* dout; long long do_sb, do_ss, do_sh;   // [B, Sq, H, D]
   void* dq; void* dk; void* dv;                  // contiguous, layouts of q / k / v
   float* delta;                                  // [B, H, Sq] fp32 workspace
   float* dslopes; float* dslope_rows;            // [H] out and [B, H, Sq] workspace, or both null
 } TfScoreAttnArgs;
-size_t tf_score_attn_work(const TfScoreAttnArgs* a);
+size_t tf_score_attn_work(int B, int Sq, int Sk, int H, int Hk, int D, int is_f32);
 int tf_score_attn_fwd(const TfScoreAttnArgs* a, tf_stream_t s);
 int tf_score_attn_bwd(const TfScoreAttnArgs* a, tf_stream_t s);
 

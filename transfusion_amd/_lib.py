@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import re
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 HEADER = os.path.join(os.path.dirname(HERE), "include", "tfusion.h")
@@ -80,6 +81,19 @@ def _parse_header(path: str):
 
 
 CONSTS, ENUMS, STRUCTS, FUNCTIONS = _parse_header(HEADER)
+
+_CODES = {C.c_void_p: "P", C.c_int: "i", C.c_uint: "I", C.c_float: "f", C.c_double: "d", C.c_longlong: "q", C.c_size_t: "N", C.c_uint64: "Q",
+          C.c_uint32: "I"}
+
+
+def packer(name: str):
+    """The ``pack`` of a flat argument struct: all its fields in the header's order -> the bytes the library reads (native alignment).
+    Filling a ctypes structure of fifty fields by keyword costs 5 us a call, this 1 us -- it matters where the call is a single token."""
+    fields = STRUCTS[name]._fields_
+    st = struct.Struct("@" + "".join(_CODES[t] for _, t in fields) + "0P")
+    if st.size != C.sizeof(STRUCTS[name]):
+        raise TfError(f"{name} does not pack to the size of its C layout")
+    return st.pack
 globals().update(STRUCTS)
 globals().update(ENUMS)
 TF_MAX_LAYERS = CONSTS["TF_MAX_LAYERS"]
@@ -135,7 +149,7 @@ def load():
     for f in ("tf_sumsq", "tf_sumsq_set"):
         getattr(lib, f).argtypes = [C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p]
     lib.tf_score_attn_work.restype = C.c_size_t
-    lib.tf_score_attn_work.argtypes = [C.c_void_p]
+    lib.tf_score_attn_work.argtypes = [C.c_int] * 7
     lib.tf_grad_clip_parts.restype = C.c_longlong
     lib.tf_grad_clip_parts.argtypes = [C.c_void_p, C.c_int]
     lib.tf_dropout_mask.argtypes = [C.c_void_p, C.c_longlong, C.c_uint32, C.c_uint32, C.c_void_p]
@@ -154,12 +168,19 @@ def check(rc: int, what: str = ""):
         raise TfError(f"{what or 'tfusion call'} failed (rc={rc}): {msg}")
 
 
-def call(fn_name: str, struct, stream: int, *extra):
+def call(fn_name: str, args_struct, stream: int, *extra):
     """Invoke an ``int fn(const Struct*, [extra ints...], tf_stream_t)`` entry."""
     lib = load()
     fn = getattr(lib, fn_name)
-    args = [C.byref(struct)] + [C.c_int(x) for x in extra] + [C.c_void_p(stream)]
+    args = [C.byref(args_struct)] + [C.c_int(x) for x in extra] + [C.c_void_p(stream)]
     check(fn(*args), fn_name)
+
+
+def call_packed(fn_name: str, packed: bytes, stream: int):
+    """``call`` of an entry whose argument struct was formed by ``packer``."""
+    rc = getattr(_lib or load(), fn_name)(packed, C.c_void_p(stream))
+    if rc:
+        check(rc, fn_name)
 
 
 def ptr(t) -> int:

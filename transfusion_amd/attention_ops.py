@@ -20,30 +20,36 @@ _POS_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
 def _heads(name, t, like=None):
-    """A [B, S, H, D] operand with strides the kernels read as they are (channels contiguous, rows on 16 bytes), copied otherwise."""
-    ops._require_cuda(t)
+    """A bf16 or fp32 [B, S, H, D] device tensor, of the type and on the device of ``like``."""
+    if not t.is_cuda:
+        ops._require_cuda(t)
     if t.dim() != 4:
         raise L.TfError(f"{name}: [batch, tokens, heads, head_dim] expected, got {tuple(t.shape)}")
-    ops._is_f32(t)
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if like is None:
+        ops._is_f32(t)
+    elif t.dtype != like.dtype or t.device != like.device:
         raise L.TfError(f"{name}: {t.dtype} on {t.device}, the queries are {like.dtype} on {like.device}")
-    return t
 
 
 def _rows(t):
-    """``t`` itself if its channels are contiguous, every row starts on 16 bytes and the rows lie within 16 MiB of each other (64 of them
-    are addressed with 32-bit offsets), else a contiguous copy."""
-    e = t.element_size()
-    if t.numel() == 0:
-        return t
-    ok = (t.shape[3] == 1 or t.stride(3) == 1) and t.data_ptr() % 16 == 0
-    ok = ok and all(t.shape[i] == 1 or t.stride(i) * e % 16 == 0 for i in range(3)) and t.stride(1) * e < 1 << 24
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
-
-
-def _strides(t):
-    """Batch, token and head strides in elements; 0 for an axis of length 1 (torch leaves any number there)."""
-    return tuple(0 if t.shape[i] == 1 else t.stride(i) for i in range(3))
+    """(tensor, batch stride, token stride, head stride): ``t`` itself if its channels are contiguous, every row starts on 16 bytes and the rows
+    lie within 16 MiB of each other (64 of them are addressed with 32-bit offsets), else a contiguous copy.  Strides in elements, 0 for
+    an axis of length 1 (torch leaves any number there)."""
+    B, S, H, D = t.shape
+    sb, ss, sh, sd = t.stride()
+    if B == 1:
+        sb = 0
+    if S == 1:
+        ss = 0
+    if H == 1:
+        sh = 0
+    n = 16 // t.element_size()
+    if (sd == 1 or D == 1) and not (sb | ss | sh) & (n - 1) and not t.data_ptr() & 15 and ss < n << 20:
+        return t, sb, ss, sh
+    if D % n == 0 or sd != 1:            # (channel counts that no 16 bytes divide: rotary takes such rows element by element, as they are)
+        t = t.clone(memory_format=torch.contiguous_format)
+        sb, ss, sh = S * H * D, H * D, D
+    return t, sb, ss, sh
 
 
 def _ints(name, t, shape, dev):
@@ -94,19 +100,28 @@ class RotaryPlan:
         self.axis = torch.tensor([a for a, n in enumerate(axes) for _ in range(n)], dtype=torch.int32).to(dev)
 
 
+_pack_rotary = L.packer("TfRotaryArgs")
+_pack_score = L.packer("TfScoreAttnArgs")
+
+
 def _rotary_call(q, k, pos, plan, inverse):
     dev = q.device
-    q, k = _rows(q), _rows(k) if k is not None else None
+    q, qb, qs, qh = _rows(q)
     B, S, H, D = q.shape
     qo = torch.empty(B, S, H, D, dtype=q.dtype, device=dev)
-    ko = None if k is None else torch.empty(B, S, k.shape[2], D, dtype=q.dtype, device=dev)
-    qs, ks = _strides(q), _strides(k) if k is not None else (0, 0, 0)
-    a = L.TfRotaryArgs(q=L.ptr(q), q_sb=qs[0], q_ss=qs[1], q_sh=qs[2], k=L.ptr(k), k_sb=ks[0], k_ss=ks[1], k_sh=ks[2], q_out=L.ptr(qo), k_out=L.ptr(ko),
-                       B=B, S=S, H=H, Hk=0 if k is None else k.shape[2], D=D, is_f32=ops._is_f32(q), pos=L.ptr(pos), pos_type=_POS_TYPES[pos.dtype],
-                       pos_batched=1 if pos.dim() == 3 else 0, n_axes=len(plan.axes), inv_freq=L.ptr(plan.freq_rev), axis=L.ptr(plan.axis),
-                       pairs=plan.pairs, interleaved=int(plan.interleaved), inverse=int(inverse))
+    if k is None:
+        kp = kb = ks = kh = Hk = kop = 0
+        ko = None
+    else:
+        k, kb, ks, kh = _rows(k)
+        Hk = k.shape[2]
+        ko = torch.empty(B, S, Hk, D, dtype=q.dtype, device=dev)
+        kp, kop = k.data_ptr(), ko.data_ptr()
+    a = _pack_rotary(q.data_ptr(), qb, qs, qh, kp, kb, ks, kh, qo.data_ptr(), kop, B, S, H, Hk, D, ops._is_f32(q),
+                     pos.data_ptr(), _POS_TYPES[pos.dtype], pos.dim() == 3, len(plan.axes), plan.freq_rev.data_ptr(), plan.axis.data_ptr(),
+                     plan.pairs, plan.interleaved, inverse)
     with ops.on_device(dev):
-        L.call("tf_rotary", a, ops._stream())
+        L.call_packed("tf_rotary", a, ops._stream())
     return qo, ko
 
 
@@ -161,29 +176,25 @@ def rotary(q, k, pos, plan: RotaryPlan):
 # ------------------------------------------------------------------------------------------------------
 # attention with changed scores
 # ------------------------------------------------------------------------------------------------------
-def _score_args(q, k, v, out, opt):
-    scale, softcap, slopes, causal, prefix, q_start, q_doc, k_doc = opt
-    B, Sq, H, D = q.shape
-    qs, ks, vs = _strides(q), _strides(k), _strides(v)
-    return L.TfScoreAttnArgs(q=L.ptr(q), q_sb=qs[0], q_ss=qs[1], q_sh=qs[2], k=L.ptr(k), k_sb=ks[0], k_ss=ks[1], k_sh=ks[2],
-                             v=L.ptr(v), v_sb=vs[0], v_ss=vs[1], v_sh=vs[2], out=L.ptr(out), B=B, Sq=Sq, Sk=k.shape[1], H=H, Hk=k.shape[2], D=D,
-                             is_f32=ops._is_f32(q), scale=scale, softcap=softcap, slopes=L.ptr(slopes), causal=causal, prefix=L.ptr(prefix),
-                             q_start=L.ptr(q_start), q_doc=L.ptr(q_doc), k_doc=L.ptr(k_doc))
-
-
 def _score_fwd(q, k, v, opt, want_lse):
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    scale, softcap, slopes, causal, prefix, q_start, q_doc, k_doc = opt
+    q, qb, qs, qh = _rows(q)
+    k, kb, ks, kh = _rows(k)
+    v, vb, vs, vh = _rows(v)
     B, Sq, H, D = q.shape
-    out = torch.empty(B, Sq, H, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, H, Sq, dtype=torch.float32, device=q.device) if want_lse else None
-    a = _score_args(q, k, v, out, opt)
-    a.lse = L.ptr(lse)
-    need = L.load().tf_score_attn_work(L.C.byref(a))
-    if need:
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
-        a.work, a.work_bytes = L.ptr(work), need
-    with ops.on_device(q.device):
-        L.call("tf_score_attn_fwd", a, ops._stream())
+    Sk, Hk = k.shape[1], k.shape[2]
+    dev = q.device
+    out = torch.empty(B, Sq, H, D, dtype=q.dtype, device=dev)
+    lse = torch.empty(B, H, Sq, dtype=torch.float32, device=dev) if want_lse else None
+    p = L.ptr
+    f32 = ops._is_f32(q)
+    need = L.load().tf_score_attn_work(B, Sq, Sk, H, Hk, D, f32)
+    work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    a = _pack_score(q.data_ptr(), qb, qs, qh, k.data_ptr(), kb, ks, kh, v.data_ptr(), vb, vs, vh, out.data_ptr(), p(lse), B, Sq, Sk, H, Hk, D, f32,
+                    scale, softcap, p(slopes), causal, p(prefix), p(q_start), p(q_doc), p(k_doc), p(work), need,
+                    0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    with ops.on_device(dev):
+        L.call_packed("tf_score_attn_fwd", a, ops._stream())
     return q, k, v, out, lse
 
 
@@ -202,19 +213,22 @@ class _ScoreAttnFn(torch.autograd.Function):
     def backward(ctx, go):
         q, k, v, slopes, out, lse, prefix, q_start, q_doc, k_doc = ctx.saved_tensors
         scale, softcap, causal = ctx.opt
-        dev = q.device
-        go = _rows(go)
-        a = _score_args(q, k, v, out, (scale, softcap, slopes, causal, prefix, q_start, q_doc, k_doc))
+        dev, p = q.device, L.ptr
+        q, qb, qs, qh = _rows(q)
+        k, kb, ks, kh = _rows(k)
+        v, vb, vs, vh = _rows(v)
+        go, gb, gs, gh = _rows(go)
+        B, Sq, H, D = q.shape
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-        delta = torch.empty_like(lse)
-        a.lse, a.delta, a.dq, a.dk, a.dv, a.dout = L.ptr(lse), L.ptr(delta), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.ptr(go)
-        a.do_sb, a.do_ss, a.do_sh = _strides(go)
-        ds = None
+        delta = torch.empty(B, H, Sq, dtype=torch.float32, device=dev)
+        ds = rows = None
         if slopes is not None and ctx.needs_input_grad[3]:
-            ds, rows = torch.empty_like(slopes), torch.empty_like(lse)
-            a.dslopes, a.dslope_rows = L.ptr(ds), L.ptr(rows)
+            ds, rows = torch.empty(H, dtype=torch.float32, device=dev), torch.empty_like(delta)
+        a = _pack_score(q.data_ptr(), qb, qs, qh, k.data_ptr(), kb, ks, kh, v.data_ptr(), vb, vs, vh, out.data_ptr(), lse.data_ptr(),
+                        B, Sq, k.shape[1], H, k.shape[2], D, ops._is_f32(q), scale, softcap, p(slopes), causal, p(prefix), p(q_start), p(q_doc),
+                        p(k_doc), 0, 0, go.data_ptr(), gb, gs, gh, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), p(ds), p(rows))
         with ops.on_device(dev):
-            L.call("tf_score_attn_bwd", a, ops._stream())
+            L.call_packed("tf_score_attn_bwd", a, ops._stream())
         return dq, dk, dv, ds, None, None, None, None, None, None, None
 
 

@@ -40,6 +40,52 @@ template <bool INF> __device__ __forceinline__ void gn_add(double& s, unsigned& 
   else s = __builtin_fma((double)x, (double)x, s);
 }
 
+// f over n values from x on (STORE: x = f(x)), by 256 threads: 16-byte accesses from the first aligned address on, four in flight a thread,
+// single elements before and behind
+template <class T, class F> __device__ __forceinline__ void gn_each(const T* xc, long long n, int tid, F&& f, bool store) {
+  constexpr int N = 16 / sizeof(T);
+  T* x = const_cast<T*>(xc);
+  auto one = [&](long long i) {
+    if constexpr (sizeof(T) == 2) { const float y = f(bf2f(x[i])); if (store) x[i] = f2bf(y); }
+    else { const float y = f(x[i]); if (store) x[i] = y; }
+  };
+  const long long head = min(n, (long long)(((16 - ((size_t)x & 15)) & 15) / sizeof(T)));
+  if (tid < head) one(tid);
+  u32x4* v = (u32x4*)(x + head);
+  const long long nv = (n - head) / N;
+  auto vec = [&](const u32x4& u) {
+    u32x4 r;
+    if constexpr (sizeof(T) == 2) {
+      float e[8];
+      unpack8(u, e);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[k] = f(e[k]);
+      r = pack8(e);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { const unsigned w = u[k]; r[k] = __builtin_bit_cast(unsigned, f(__builtin_bit_cast(float, w))); }
+    }
+    return r;
+  };
+  long long i = tid;
+  for (; i + 3 * 256 < nv; i += 4 * 256) {
+    u32x4 u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u[k] = v[i + k * 256];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const u32x4 r = vec(u[k]);
+      if (store) v[i + k * 256] = r;
+    }
+  }
+  for (; i < nv; i += 256) {
+    const u32x4 r = vec(v[i]);
+    if (store) v[i] = r;
+  }
+  const long long t0 = head + nv * N;
+  if (t0 + tid < n) one(t0 + tid);
+}
+
 template <bool INF> __device__ __forceinline__ double gn_block_reduce(double s, unsigned m, double* sh) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -63,13 +109,8 @@ __global__ __launch_bounds__(256) void grad_norm_part_kernel(const GnTab tab, in
   const long long lo = b * chunk, hi = min(tab.n[t], lo + chunk);
   double s = 0.0;
   unsigned m = 0u;
-  if (bf) {
-    const u16* x = (const u16*)tab.p[t];
-    for (long long i = lo + tid; i < hi; i += 256) gn_add<INF>(s, m, bf2f(x[i]));
-  } else {
-    const float* x = (const float*)tab.p[t];
-    for (long long i = lo + tid; i < hi; i += 256) gn_add<INF>(s, m, x[i]);
-  }
+  if (bf) gn_each<u16>((const u16*)tab.p[t] + lo, hi - lo, tid, [&](float x) { gn_add<INF>(s, m, x); return x; }, false);
+  else gn_each<float>((const float*)tab.p[t] + lo, hi - lo, tid, [&](float x) { gn_add<INF>(s, m, x); return x; }, false);
   const double r = gn_block_reduce<INF>(s, m, sh);
   if (tid == 0) part[blockIdx.x] = r;
 }
@@ -93,17 +134,13 @@ __global__ __launch_bounds__(256) void grad_clip_kernel(const GnTab tab, int cou
   float coef = max_norm / (total + 1e-6f);
   if (coef > 1.0f) coef = 1.0f;                          // (a NaN stays)
   if (coef == 1.0f) return;                              // times one is the same bits: nothing to write
-  const int t = gn_find(tab, count, (int)blockIdx.x);
+  const int blk = (int)(gridDim.x - 1 - blockIdx.x);     // from the end: what the first pass read last is still in the caches
+  const int t = gn_find(tab, count, blk);
   const bool bf = tab.blk0[t] < 0;
-  const long long b = (long long)((int)blockIdx.x - (tab.blk0[t] & 0x7fffffff));
+  const long long b = (long long)(blk - (tab.blk0[t] & 0x7fffffff));
   const long long lo = b * chunk, hi = min(tab.n[t], lo + chunk);
-  if (bf) {
-    u16* x = (u16*)tab.p[t];
-    for (long long i = lo + tid; i < hi; i += 256) x[i] = f2bf(bf2f(x[i]) * coef);
-  } else {
-    float* x = (float*)tab.p[t];
-    for (long long i = lo + tid; i < hi; i += 256) x[i] *= coef;
-  }
+  if (bf) gn_each<u16>((const u16*)tab.p[t] + lo, hi - lo, tid, [&](float x) { return x * coef; }, true);
+  else gn_each<float>((const float*)tab.p[t] + lo, hi - lo, tid, [&](float x) { return x * coef; }, true);
 }
 
 struct GnPlan {

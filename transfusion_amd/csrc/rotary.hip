@@ -9,6 +9,7 @@
 // write of the rows, which is its floor.
 #include "tf_common.h"
 #include "tf_kernels.h"
+#include <algorithm>
 
 namespace {
 
@@ -40,93 +41,99 @@ __device__ __forceinline__ double rot_pos(const TfRotaryArgs& a, size_t i) {
   return (double)((const float*)a.pos)[i];
 }
 
-// tt tokens of the [B * S] per workgroup; VEC: 16-byte accesses (the launcher checked alignment and that no pair straddles two vectors)
+// n / d for n < 2^16 (m = ceil(2^32 / d), d < 2^16): one high multiplication
+__device__ __forceinline__ int div16(int n, unsigned m) { return (int)__umulhi((unsigned)n, m); }
+unsigned div16_of(int d) { return d == 1 ? 0u : (unsigned)((0x100000000ull + d - 1) / d); }
+struct RotGeo {
+  int tt;                      // tokens of a workgroup; tt * (H + Hk) * units < 2^16
+  int units;                   // pieces of a head's row (see the kernel)
+  int Pp;                      // pairs, rounded up to 4: the tables' row length
+  unsigned m_units, m_heads, m_pairs;
+};
+__device__ __forceinline__ int div_u(int n, int d, unsigned m) { return d == 1 ? n : div16(n, m); }
+
+// A workgroup turns g.tt tokens of the [B * S]: the table of their angles first, then pieces of rows, neighbours in memory by neighbouring
+// threads.  VEC: a piece is a 16-byte vector of an interleaved row, or the two vectors of a row's halves that turn together, or a vector
+// that passes through (the launcher checked that no pair straddles vectors); else one pair or one channel.
 template <bool F32, bool VEC>
-__global__ __launch_bounds__(256) void rotary_kernel(const TfRotaryArgs a, int tt) {
+__global__ __launch_bounds__(256) void rotary_kernel(const TfRotaryArgs a, const RotGeo g) {
   using V = RVec<F32>;
+  constexpr int N = V::N;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  float* cs = (float*)smem;                              // [tt][2][P]: cosines, then sines, of a token
-  const int P = a.pairs, tid = threadIdx.x;
-  const long long tokens = (long long)a.B * a.S, t0 = (long long)blockIdx.x * tt;
-  const int nt = (int)min((long long)tt, tokens - t0);
+  const int P = a.pairs, Pp = g.Pp, tid = threadIdx.x, HT = a.H + a.Hk;
+  long long* tq = (long long*)smem;                      // [tt] offsets of the token's first Q row / K row, in elements
+  long long* tk = tq + g.tt;
+  float* cs = (float*)(tk + g.tt);                       // [tt][2][Pp]: cosines, then sines
+  const long long tokens = (long long)a.B * a.S, t0 = (long long)blockIdx.x * g.tt;
+  const int nt = (int)min((long long)g.tt, tokens - t0);
+  if (tid < nt) {
+    const long long tok = t0 + tid, b = tok / a.S, s = tok - b * a.S;
+    tq[tid] = b * a.q_sb + s * a.q_ss;
+    tk[tid] = b * a.k_sb + s * a.k_ss;
+  }
   for (int i = tid; i < nt * P; i += 256) {
-    const int t = i / P, p = i % P;
+    const int t = div_u(i, P, g.m_pairs), p = i - t * P;
     const long long tok = t0 + t;
     const size_t row = a.pos_batched ? (size_t)tok : (size_t)(tok % a.S);
     const double rev = rot_pos(a, row * a.n_axes + a.axis[p]) * a.inv_freq[p];
     float s, c;
     sincospif(2.0f * (float)(rev - rint(rev)), &s, &c);
-    cs[2 * t * P + p] = c;
-    cs[(2 * t + 1) * P + p] = a.inverse ? -s : s;
+    cs[2 * t * Pp + p] = c;
+    cs[(2 * t + 1) * Pp + p] = a.inverse ? -s : s;
   }
   __syncthreads();
-  const int HT = a.H + a.Hk;
-  if (VEC) {
-    constexpr int N = V::N;
-    // units of a head's row: interleaved: every vector by itself; halves: the P / N pairs of vectors, then the vectors that pass through
-    const int units = a.interleaved ? a.D / N : P / N + (a.D - 2 * P) / N;
-    for (int i = tid; i < nt * HT * units; i += 256) {
-      const int u = i % units, h = i / units % HT, t = i / units / HT;
-      const long long tok = t0 + t;
-      const size_t b = (size_t)(tok / a.S), s = (size_t)(tok % a.S);
-      const bool isq = h < a.H;
-      const int hh = isq ? h : h - a.H;
-      const void* x = isq ? a.q : a.k;
-      void* y = isq ? a.q_out : a.k_out;
-      const size_t xo = isq ? b * a.q_sb + s * a.q_ss + (size_t)hh * a.q_sh : b * a.k_sb + s * a.k_ss + (size_t)hh * a.k_sh;
-      const size_t yo = ((size_t)tok * (isq ? a.H : a.Hk) + hh) * a.D;
-      const float* c = cs + 2 * t * P;
-      const float* sn = c + P;
-      float f[N], g[N];
+  const int W = HT * g.units;
+#pragma unroll 2
+  for (int i = tid; i < nt * W; i += 256) {
+    const int th = div_u(i, g.units, g.m_units), u = i - th * g.units, t = div_u(th, HT, g.m_heads), h = th - t * HT;
+    const bool isq = h < a.H;
+    const int hh = isq ? h : h - a.H;
+    const void* x = isq ? a.q : a.k;
+    void* y = isq ? a.q_out : a.k_out;
+    const size_t xo = isq ? tq[t] + hh * a.q_sh : tk[t] + hh * a.k_sh;
+    const size_t yo = ((size_t)(t0 + t) * (isq ? a.H : a.Hk) + hh) * a.D;
+    const float* c = cs + 2 * t * Pp;
+    const float* sn = c + Pp;
+    if (VEC) {
+      float f[N], w[N];
       if (a.interleaved) {
         V::load(x, xo + u * N, f);
 #pragma unroll
         for (int e = 0; e < N / 2; ++e) {
-          const int p = u * (N / 2) + e;
-          const float cc = p < P ? c[p] : 1.f, ss = p < P ? sn[p] : 0.f;
-          g[2 * e] = p < P ? f[2 * e] * cc - f[2 * e + 1] * ss : f[2 * e];
-          g[2 * e + 1] = p < P ? f[2 * e] * ss + f[2 * e + 1] * cc : f[2 * e + 1];
+          const int p = u * (N / 2) + e, pc = min(p, P - 1);
+          const float cc = c[pc], ss = sn[pc];
+          w[2 * e] = p < P ? f[2 * e] * cc - f[2 * e + 1] * ss : f[2 * e];
+          w[2 * e + 1] = p < P ? f[2 * e] * ss + f[2 * e + 1] * cc : f[2 * e + 1];
         }
-        V::store(y, yo + u * N, g);
-      } else if (u < P / N) {
+        V::store(y, yo + u * N, w);
+      } else if (u * N < P) {
         V::load(x, xo + u * N, f);
-        V::load(x, xo + P + u * N, g);
+        V::load(x, xo + P + u * N, w);
         float r0[N], r1[N];
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float cc = c[u * N + e], ss = sn[u * N + e];
-          r0[e] = f[e] * cc - g[e] * ss;
-          r1[e] = f[e] * ss + g[e] * cc;
+        for (int e = 0; e < N; e += 4) {
+          const f32x4 cc = *(const f32x4*)(c + u * N + e), ss = *(const f32x4*)(sn + u * N + e);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            r0[e + k] = f[e + k] * cc[k] - w[e + k] * ss[k];
+            r1[e + k] = f[e + k] * ss[k] + w[e + k] * cc[k];
+          }
         }
         V::store(y, yo + u * N, r0);
         V::store(y, yo + P + u * N, r1);
       } else {
-        const int c0 = 2 * P + (u - P / N) * N;
+        const int c0 = P + u * N;
         V::load(x, xo + c0, f);
         V::store(y, yo + c0, f);
       }
-    }
-  } else {
-    const int units = a.D - P;                           // P pairs, D - 2 P channels that pass through
-    for (int i = tid; i < nt * HT * units; i += 256) {
-      const int u = i % units, h = i / units % HT, t = i / units / HT;
-      const long long tok = t0 + t;
-      const size_t b = (size_t)(tok / a.S), s = (size_t)(tok % a.S);
-      const bool isq = h < a.H;
-      const int hh = isq ? h : h - a.H;
-      const void* x = isq ? a.q : a.k;
-      void* y = isq ? a.q_out : a.k_out;
-      const size_t xo = isq ? b * a.q_sb + s * a.q_ss + (size_t)hh * a.q_sh : b * a.k_sb + s * a.k_ss + (size_t)hh * a.k_sh;
-      const size_t yo = ((size_t)tok * (isq ? a.H : a.Hk) + hh) * a.D;
-      if (u < P) {
-        const float c = cs[2 * t * P + u], sn = cs[(2 * t + 1) * P + u];
-        const int c0 = a.interleaved ? 2 * u : u, c1 = a.interleaved ? 2 * u + 1 : P + u;
-        const float f = V::get(x, xo + c0), g = V::get(x, xo + c1);
-        V::put(y, yo + c0, f * c - g * sn);
-        V::put(y, yo + c1, f * sn + g * c);
-      } else {
-        V::put(y, yo + P + u, V::get(x, xo + P + u));
-      }
+    } else if (u < P) {
+      const float cc = c[u], ss = sn[u];
+      const int c0 = a.interleaved ? 2 * u : u, c1 = a.interleaved ? 2 * u + 1 : P + u;
+      const float f = V::get(x, xo + c0), w = V::get(x, xo + c1);
+      V::put(y, yo + c0, f * cc - w * ss);
+      V::put(y, yo + c1, f * ss + w * cc);
+    } else {
+      V::put(y, yo + P + u, V::get(x, xo + P + u));
     }
   }
 }
@@ -149,13 +156,23 @@ extern "C" int tf_launch_rotary(const TfRotaryArgs* a, hipStream_t st) {
   bool vec = a->D % n == 0 && (a->interleaved || a->pairs % n == 0);
   if (a->H > 0) vec = vec && vec_ok(a->q, a->q_out, a->q_sb, a->q_ss, a->q_sh, n);
   if (a->Hk > 0) vec = vec && vec_ok(a->k, a->k_out, a->k_sb, a->k_ss, a->k_sh, n);
-  const int tt = 4;
+  RotGeo g;
+  g.units = vec ? (a->interleaved ? a->D / n : (a->D - a->pairs) / n) : a->D - a->pairs;
+  g.Pp = (a->pairs + 3) / 4 * 4;
+  const long long W = (long long)HT * g.units;
+  if (W > 0xffff || a->D > 0xffff) return -5;
+  // eight pieces a thread where that still leaves four workgroups a CU, fewer tokens a workgroup otherwise; the tables stay in 16 KiB
+  long long tt = std::max(1ll, std::min({2048 / W, tokens / 1024, 0xffff / std::max<long long>(W, a->pairs), 2048ll / g.Pp, 64ll}));
+  g.tt = (int)tt;
+  g.m_units = div16_of(g.units);
+  g.m_heads = div16_of(HT);
+  g.m_pairs = div16_of(a->pairs);
   const long long blocks = (tokens + tt - 1) / tt;
   if (blocks > 0x7fffffffll) return -4;
-  const size_t lds = (size_t)tt * 2 * a->pairs * sizeof(float);
+  const size_t lds = (size_t)tt * (16 + 2 * g.Pp * sizeof(float));
   const double bytes = 2.0 * tokens * HT * a->D * (a->is_f32 ? 4 : 2);
   TfTraceScope tr("rotary_kernel", st, 3.0 * tokens * HT * 2 * a->pairs, bytes);
-  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, *a, tt); };
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(256), lds, st, *a, g); };
   if (a->is_f32) vec ? go(rotary_kernel<true, true>) : go(rotary_kernel<true, false>);
   else vec ? go(rotary_kernel<false, true>) : go(rotary_kernel<false, false>);
   return (int)hipGetLastError();

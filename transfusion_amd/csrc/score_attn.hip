@@ -975,28 +975,48 @@ __global__ __launch_bounds__(256, 1) void score_few32_kernel(const TfScoreAttnAr
   few_finish<true, DB>(a, w, b, kvh, m_run, l_run, o, (float*)smem, nsplit, split, wave, lane);
 }
 
-// joins the parts of a split forward: one wave a row, four channels a lane
+// joins the parts of a split forward, one workgroup a row: the parts' weights first (one thread a part), then every wave adds up a quarter
+// of the parts (four channels a lane, the loads of several parts in flight).  At 32 parts of 64 rows a wave that walked all parts by
+// itself took 23 us, as long as the product; this form takes 5.
+constexpr int JOIN_MAX = 512;
 template <bool F32> __global__ __launch_bounds__(256) void score_join_kernel(const TfScoreAttnArgs a, int nsplit) {
-  const long long rows = (long long)a.B * a.H * a.Sq, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (row >= rows) return;
+  __shared__ float wgt[JOIN_MAX], red[8];
+  __shared__ f32x4 part[256];
+  const long long rows = (long long)a.B * a.H * a.Sq, row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* po = (const float*)a.work + row * a.D;
   const float* pml = (const float*)a.work + (long long)nsplit * rows * a.D + row * 2;
   float mx = S_NEG;
-  for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, pml[(long long)s * rows * 2]);
+  for (int s = tid; s < nsplit; s += 256) mx = fmaxf(mx, pml[(long long)s * rows * 2]);
+  mx = wave_max(mx);
+  if (lane == 0) red[wave] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   float l = 0.f;
-  f32x4 acc = {0, 0, 0, 0};
-  for (int s = 0; s < nsplit; ++s) {
+  for (int s = tid; s < nsplit; s += 256) {
     const float w = fast_exp2(pml[(long long)s * rows * 2] - mx);
+    wgt[s] = w;
     l += w * pml[(long long)s * rows * 2 + 1];
-    if (lane * 4 < a.D) acc += w * *(const f32x4*)(po + (long long)s * rows * a.D + lane * 4);
   }
+  l = wave_sum(l);
+  if (lane == 0) red[4 + wave] = l;
+  __syncthreads();
+  l = (red[4] + red[5]) + (red[6] + red[7]);
+  f32x4 acc = {0, 0, 0, 0};
+  if (lane * 4 < a.D) {
+#pragma unroll 8
+    for (int s = wave; s < nsplit; s += 4) acc += wgt[s] * *(const f32x4*)(po + (long long)s * rows * a.D + lane * 4);
+  }
+  part[tid] = acc;
+  __syncthreads();
+  if (wave != 0) return;
+  acc = (part[lane] + part[64 + lane]) + (part[128 + lane] + part[192 + lane]);
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   const int i = (int)(row % a.Sq), bh = (int)(row / a.Sq), b = bh / a.H, head = bh % a.H;
   const long long oo = (((long long)b * a.Sq + i) * a.H + head) * a.D + lane * 4;
   if (lane * 4 < a.D) {
     if constexpr (F32) *(f32x4*)((float*)a.out + oo) = acc * inv;
-    else *(u32x2*)((u16*)a.out + oo) = u32x2{pack2bf(acc[0] * inv, acc[1] * inv), pack2bf(acc[2] * inv, acc[3] * inv)};
+    else *(u32x2*)((u16*)a.out + oo) = u32x2{pk2(acc[0] * inv, acc[1] * inv), pk2(acc[2] * inv, acc[3] * inv)};
   }
   if (lane == 0 && a.lse != nullptr) a.lse[row] = l == 0.f ? INFINITY : mx + log2f(l);
 }
@@ -1627,7 +1647,7 @@ template <bool F32, int HDP> int launch_fwd(const TfScoreAttnArgs* a, hipStream_
   }
   if (f.nsplit > 1) {
     TfTraceScope tr("score_join_kernel", st);
-    hipLaunchKernelGGL(score_join_kernel<F32>, dim3((unsigned)(((long long)a->B * a->H * a->Sq + 3) / 4)), dim3(256), 0, st, *a, f.nsplit);
+    hipLaunchKernelGGL(score_join_kernel<F32>, dim3((unsigned)((long long)a->B * a->H * a->Sq)), dim3(256), 0, st, *a, f.nsplit);
   }
   return (int)hipGetLastError();
 }
@@ -1682,10 +1702,16 @@ template <class Fn> int by_head_dim(const TfScoreAttnArgs* a, Fn&& fn) {
 }  // namespace
 
 // bytes of TfScoreAttnArgs.work for the forward; the backward needs none
-extern "C" size_t tf_score_attn_work(const TfScoreAttnArgs* a) {
+static size_t work_bytes(const TfScoreAttnArgs* a) {
   if (check(a) != 0 || a->B == 0 || a->Sq == 0) return 0;
   const FwdPlan f = fwd_plan(a);
   return f.nsplit > 1 ? (size_t)f.nsplit * a->B * a->H * a->Sq * (a->D + 2) * sizeof(float) : 0;
+}
+
+extern "C" size_t tf_score_attn_work(int B, int Sq, int Sk, int H, int Hk, int D, int is_f32) {
+  TfScoreAttnArgs a{};
+  a.B = B; a.Sq = Sq; a.Sk = Sk; a.H = H; a.Hk = Hk; a.D = D; a.is_f32 = is_f32;
+  return work_bytes(&a);
 }
 
 extern "C" int tf_launch_score_fwd(const TfScoreAttnArgs* a, hipStream_t st) {
@@ -1696,7 +1722,7 @@ extern "C" int tf_launch_score_fwd(const TfScoreAttnArgs* a, hipStream_t st) {
   if (a->q == nullptr || a->out == nullptr || (a->Sk > 0 && (a->k == nullptr || a->v == nullptr))) return -6;
   if (!aligned(a->q, a->q_sb, a->q_ss, a->q_sh, e) || !aligned(a->k, a->k_sb, a->k_ss, a->k_sh, e) || !aligned(a->v, a->v_sb, a->v_ss, a->v_sh, e) ||
       !aligned(a->out, 0, 0, 0, e)) return -7;
-  const size_t need = tf_score_attn_work(a);
+  const size_t need = work_bytes(a);
   if (need > 0 && (a->work == nullptr || a->work_bytes < need || ((uintptr_t)a->work & 15) != 0)) return -8;
   return by_head_dim(a, [&](auto f32, auto hdp) { return launch_fwd<decltype(f32)::value, decltype(hdp)::value>(a, st); });
 }

@@ -34,6 +34,9 @@ def radam_schedule(step: int, beta1: float, beta2: float, degenerated_to_sgd: bo
     return n_sma, -1.0, 0
 
 
+_CLIP_TYPES = {torch.float32, torch.bfloat16}
+
+
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0):
     """``torch.nn.utils.clip_grad_norm_`` on the device, over any number of separate gradient tensors (tf_grad_clip): returns the norm over
     all of them as a 0-d fp32 device tensor (no host synchronisation) and multiplies every gradient by ``min(1, max_norm / (norm + 1e-6))``
@@ -47,27 +50,24 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0):
         raise L.TfError(f"clip_grad_norm_: norm_type {norm_type} is not supported (2 or inf)")
     if not max_norm >= 0.0:
         raise L.TfError(f"clip_grad_norm_: max_norm {max_norm} must not be negative")
-    grads, seen = [], set()
-    for p in parameters:
-        g = p.grad
-        if g is None or id(g) in seen:
-            continue
-        seen.add(id(g))
-        grads.append(g)
+    grads = list({id(g): g for g in [p.grad for p in parameters] if g is not None}.values())
     if not grads:
         return torch.tensor(0.0)
     dev = grads[0].device
     n = len(grads)
-    ptrs, lens, bf = (L.C.c_void_p * n)(), (L.C.c_longlong * n)(), (L.C.c_int * n)()
-    for i, g in enumerate(grads):
-        if not g.is_cuda:
-            ops._require_cuda(g)
-        if g.device != dev or g.layout != torch.strided:
-            raise L.TfError("clip_grad_norm_: dense gradients on one device expected")
-        bf[i] = 1 - ops._is_f32(g)
+    if dev.type != "cuda":
+        ops._require_cuda(*grads)
+    if any([g.device != dev for g in grads]) or any([g.layout != torch.strided for g in grads]):
+        raise L.TfError("clip_grad_norm_: dense gradients on one device expected")
+    types = [g.dtype for g in grads]
+    if not _CLIP_TYPES.issuperset(types):
+        raise L.TfError(f"clip_grad_norm_: gradients of {set(types)}: fp32 or bf16 expected")
+    for g in grads:
         if not g.is_contiguous() and not torch.ops.aten.is_non_overlapping_and_dense(g):
             raise L.TfError(f"clip_grad_norm_: a gradient of shape {tuple(g.shape)} and strides {g.stride()} has gaps or overlaps itself")
-        ptrs[i], lens[i] = g.data_ptr(), g.numel()
+    ptrs = (L.C.c_void_p * n)(*[g.data_ptr() for g in grads])
+    lens = (L.C.c_longlong * n)(*[g.numel() for g in grads])
+    bf = (L.C.c_int * n)(*[t is torch.bfloat16 for t in types])
     parts = L.load().tf_grad_clip_parts(lens, n)
     work = torch.empty(max(parts, 1), dtype=torch.float64, device=dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
