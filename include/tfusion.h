@@ -628,14 +628,17 @@ typedef struct TfScoreAttnArgs {
   const float* slopes;                           // [H] fp32 or null
   int causal; const int* prefix; const int* q_start;   // [B] int32 device arrays or null
   const int* q_doc; const int* k_doc;            // [B, Sq] / [B, Sk] int32 contiguous, both or neither
-  void* work; size_t work_bytes;                 // forward: tf_score_attn_work(sizes) bytes (0: none needed)
+  void* work; size_t work_bytes;                 // tf_score_attn_work(sizes) bytes in the forward, tf_score_attn_bwd_work(sizes) in the backward
+  void* out_lo;                                  // bf16, optional: [B, Sq, H, D], what the rounding of out took; the forward writes it, the
+                                                 // backward forms rowsum(dO o) with it (else the gradients carry out's rounding a second time)
   // backward (lse from the forward)
   const void* dout; long long do_sb, do_ss, do_sh;   // [B, Sq, H, D]
   void* dq; void* dk; void* dv;                  // contiguous, layouts of q / k / v
   float* delta;                                  // [B, H, Sq] fp32 workspace
-  float* dslopes; float* dslope_rows;            // [H] out and [B, H, Sq] workspace, or both null
+  float* dslopes;                                // [H] out, or null
 } TfScoreAttnArgs;
 size_t tf_score_attn_work(int B, int Sq, int Sk, int H, int Hk, int D, int is_f32);
+size_t tf_score_attn_bwd_work(int B, int Sq, int Sk, int H, int Hk, int D, int is_f32, int dslopes);
 int tf_score_attn_fwd(const TfScoreAttnArgs* a, tf_stream_t s);
 int tf_score_attn_bwd(const TfScoreAttnArgs* a, tf_stream_t s);
 

@@ -55,7 +55,7 @@ def test_score_attn_fwd_entry_refuses(lib, kw):
 
 
 @pytest.mark.parametrize("kw", BOTH + [dict(lse=0), dict(delta=0), dict(dout=0), dict(dq=0), dict(dk=0), dict(dv=0), dict(do_ss=4), dict(dk=PTR + 4),
-                                       dict(dslopes=PTR, dslope_rows=PTR), dict(dslopes=PTR, slopes=PTR)])
+                                       dict(dslopes=PTR), dict(dslopes=PTR, slopes=PTR), dict(Hk=1, Sq=900, work=PTR, work_bytes=64), dict(out_lo=PTR + 8)])
 def test_score_attn_bwd_entry_refuses(lib, kw):
     a = attn_args(**kw)
     assert lib.tf_score_attn_bwd(C.byref(a), None) < 0

@@ -9,7 +9,7 @@ python -m transfusion_amd.build >/dev/null
 obj=$out/${src%.hip}.o
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -fPIC -std=c++17 -munsafe-fp-atomics -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops -DTF_EXPERIMENTS "$@" -c transfusion_amd/csrc/$src -o $obj
 objs=""
-for f in gemm_bf16 wgrad_multi attn_bf16 attn_x3 score_attn rotary gradnorm rowops heads comm tf_api; do
+for f in gemm_bf16 wgrad_multi attn_bf16 attn_x3 score_attn_fwd score_attn_bwd rotary gradnorm rowops heads comm tf_api; do
   if [ "$f.hip" == "$src" ]; then objs="$objs $obj"; else objs="$objs transfusion_amd/csrc/_obj/$f.o"; fi
 done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $out/libtfusion_hip.so $objs -ldl

@@ -13,7 +13,7 @@ for spec in "$@"; do
   built[${src%.hip}]=$obj
 done
 objs=""
-for f in gemm_bf16 wgrad_multi attn_bf16 attn_x3 score_attn rotary gradnorm rowops heads comm tf_api; do
+for f in gemm_bf16 wgrad_multi attn_bf16 attn_x3 score_attn_fwd score_attn_bwd rotary gradnorm rowops heads comm tf_api; do
   if [ -n "${built[$f]}" ]; then objs="$objs ${built[$f]}"; else objs="$objs transfusion_amd/csrc/_obj/$f.o"; fi
 done
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o $out/libtfusion_hip.so $objs -ldl

@@ -150,6 +150,8 @@ def load():
         getattr(lib, f).argtypes = [C.c_void_p, C.c_longlong, C.c_void_p, C.c_void_p]
     lib.tf_score_attn_work.restype = C.c_size_t
     lib.tf_score_attn_work.argtypes = [C.c_int] * 7
+    lib.tf_score_attn_bwd_work.restype = C.c_size_t
+    lib.tf_score_attn_bwd_work.argtypes = [C.c_int] * 8
     lib.tf_grad_clip_parts.restype = C.c_longlong
     lib.tf_grad_clip_parts.argtypes = [C.c_void_p, C.c_int]
     lib.tf_dropout_mask.argtypes = [C.c_void_p, C.c_longlong, C.c_uint32, C.c_uint32, C.c_void_p]

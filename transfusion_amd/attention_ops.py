@@ -185,33 +185,36 @@ def _score_fwd(q, k, v, opt, want_lse):
     Sk, Hk = k.shape[1], k.shape[2]
     dev = q.device
     out = torch.empty(B, Sq, H, D, dtype=q.dtype, device=dev)
-    lse = torch.empty(B, H, Sq, dtype=torch.float32, device=dev) if want_lse else None
     p = L.ptr
     f32 = ops._is_f32(q)
+    lse = out_lo = None
+    if want_lse:                          # for the backward: the log-sum-exps, and what the rounding of a bf16 output took
+        lse = torch.empty(B, H, Sq, dtype=torch.float32, device=dev)
+        out_lo = None if f32 else torch.empty_like(out)
     need = L.load().tf_score_attn_work(B, Sq, Sk, H, Hk, D, f32)
     work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     a = _pack_score(q.data_ptr(), qb, qs, qh, k.data_ptr(), kb, ks, kh, v.data_ptr(), vb, vs, vh, out.data_ptr(), p(lse), B, Sq, Sk, H, Hk, D, f32,
-                    scale, softcap, p(slopes), causal, p(prefix), p(q_start), p(q_doc), p(k_doc), p(work), need,
-                    0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+                    scale, softcap, p(slopes), causal, p(prefix), p(q_start), p(q_doc), p(k_doc), p(work), need, p(out_lo),
+                    0, 0, 0, 0, 0, 0, 0, 0, 0)
     with ops.on_device(dev):
         L.call_packed("tf_score_attn_fwd", a, ops._stream())
-    return q, k, v, out, lse
+    return q, k, v, out, lse, out_lo
 
 
 class _ScoreAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, scale, softcap, causal, prefix, q_start, q_doc, k_doc):
         opt = (scale, softcap, slopes, causal, prefix, q_start, q_doc, k_doc)
-        q, k, v, out, lse = _score_fwd(q, k, v, opt, True)
+        q, k, v, out, lse, out_lo = _score_fwd(q, k, v, opt, True)
         _keep(q.device, q, k, v, slopes, prefix, q_start, q_doc, k_doc)
-        ctx.save_for_backward(q, k, v, slopes, out, lse, prefix, q_start, q_doc, k_doc)
+        ctx.save_for_backward(q, k, v, slopes, out, lse, out_lo, prefix, q_start, q_doc, k_doc)
         ctx.opt = (scale, softcap, causal)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, go):
-        q, k, v, slopes, out, lse, prefix, q_start, q_doc, k_doc = ctx.saved_tensors
+        q, k, v, slopes, out, lse, out_lo, prefix, q_start, q_doc, k_doc = ctx.saved_tensors
         scale, softcap, causal = ctx.opt
         dev, p = q.device, L.ptr
         q, qb, qs, qh = _rows(q)
@@ -221,12 +224,13 @@ class _ScoreAttnFn(torch.autograd.Function):
         B, Sq, H, D = q.shape
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
         delta = torch.empty(B, H, Sq, dtype=torch.float32, device=dev)
-        ds = rows = None
-        if slopes is not None and ctx.needs_input_grad[3]:
-            ds, rows = torch.empty(H, dtype=torch.float32, device=dev), torch.empty_like(delta)
+        ds = torch.empty(H, dtype=torch.float32, device=dev) if slopes is not None and ctx.needs_input_grad[3] else None
+        f32 = ops._is_f32(q)
+        need = L.load().tf_score_attn_bwd_work(B, Sq, k.shape[1], H, k.shape[2], D, f32, ds is not None)
+        work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         a = _pack_score(q.data_ptr(), qb, qs, qh, k.data_ptr(), kb, ks, kh, v.data_ptr(), vb, vs, vh, out.data_ptr(), lse.data_ptr(),
-                        B, Sq, k.shape[1], H, k.shape[2], D, ops._is_f32(q), scale, softcap, p(slopes), causal, p(prefix), p(q_start), p(q_doc),
-                        p(k_doc), 0, 0, go.data_ptr(), gb, gs, gh, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), p(ds), p(rows))
+                        B, Sq, k.shape[1], H, k.shape[2], D, f32, scale, softcap, p(slopes), causal, p(prefix), p(q_start), p(q_doc),
+                        p(k_doc), p(work), need, p(out_lo), go.data_ptr(), gb, gs, gh, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), p(ds))
         with ops.on_device(dev):
             L.call_packed("tf_score_attn_bwd", a, ops._stream())
         return dq, dk, dv, ds, None, None, None, None, None, None, None

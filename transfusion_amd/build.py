@@ -11,9 +11,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libtfusion_hip.so")
-SOURCES = ["gemm_bf16.hip", "wgrad_multi.hip", "attn_bf16.hip", "attn_x3.hip", "score_attn.hip", "rotary.hip", "gradnorm.hip",
+SOURCES = ["gemm_bf16.hip", "wgrad_multi.hip", "attn_bf16.hip", "attn_x3.hip", "score_attn_fwd.hip", "score_attn_bwd.hip", "rotary.hip", "gradnorm.hip",
            "rowops.hip", "heads.hip", "comm.hip", "tf_api.hip"]
-HEADERS = ["tf_common.h", "tf_kernels.h", "attn_common.h", os.path.join("..", "..", "include", "tfusion.h")]
+HEADERS = ["tf_common.h", "tf_kernels.h", "attn_common.h", "score_attn.h", os.path.join("..", "..", "include", "tfusion.h")]
 # (no packed fp32 instructions: some v_pk_*_f32 forms have returned wrong values now and then on this hardware, without an error; the
 # compiler forms them by itself from ordinary float code)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-munsafe-fp-atomics", "-Wno-unused-result",

@@ -1,0 +1,495 @@
+// Backward of attention with changed scores (score_attn.h has the mathematics).  With P formed again from the log-sum-exp:
+//   dV = P^T dO ;  dP = dO V^T ;  dS = P (dP - delta), delta = rowsum(dO o) ;  dslope = -sum dS |p - j| ;  dS *= 1 - tanh^2 ;
+//   dQ = scale dS K ;  dK = scale dS^T Q .
+// Two kernels, each with every score of its own rows or keys: seven products where five would do, but no gradient is touched by two
+// workgroups, nothing is atomic, and the [Sq, Sk] tensor dS stays out of memory.
+#include "score_attn.h"
+
+namespace {
+
+// Two 32-row tiles that are used together (K and V, or Q and dO) as one image: waves 0 and 1 fetch the first, 2 and 3 the second.  Three
+// images: two pairs are under way while one is worked on, one barrier a pair; a wave waits for its own transfers of the older pair by
+// count (a pair is NI of them, everything else it issues in between only makes the wait longer).  fp32 heads of 256 have room for two.
+template <bool F32, int HDP> struct Pair {
+  using Dma = SDma<F32, HDP, 32, 2>;
+  static constexpr int HALF = Dma::BYTES, BUF = 2 * HALF, NB = F32 && HDP > 192 ? 2 : 3, IMAGES = NB * BUF;
+  // the pair in hand is there (younger, with three images: another one is under way behind it), and every wave is done with the one before
+  static __device__ __forceinline__ void wait(bool younger) {
+    if (NB == 3 && younger) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(Dma::NI) : "memory");
+    else dma_wait_barrier();
+  }
+  static __device__ __forceinline__ int after(int image) { return image + 1 == NB ? 0 : image + 1; }
+};
+
+// a pair under way: half-tile number (-1: none), full (see TileWalk)
+struct Coming { int s = -1; bool full = false; };
+
+// A workgroup's part of the rows: parts [nsplit] of fp32 in the layout of the result, added up by score_sum_kernel
+template <bool F32, int DB> __device__ __forceinline__ void store_grad(void* out, float* parts, long long n, int split, int nsplit, long long off,
+                                                                       const f32x16 (&x)[DB], float scale, int h, int D, bool ok) {
+  if (nsplit > 1) {
+    if (ok) store_part<DB>(parts, split * n + off, x, h, D);
+  } else {
+    store_row<F32, DB>(out, off, x, scale, h, D, ok);
+  }
+}
+
+// where the parts of the three gradients and of the slopes' row sums lie in the workspace
+struct BwdPlan {
+  int nqb, nkb, sq, sg, sk;              // splits of dq (keys); of dk / dv: groups of heads x ranges of queries
+  size_t o_dk, o_dv, o_rows, floats;
+};
+
+// ================================================================================================
+// dq: query on the lane, 128 queries a workgroup; also delta, and the slopes' row sums
+// ================================================================================================
+template <bool F32, int HDP, bool DOC>
+__global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_dq_kernel(const TfScoreAttnArgs a, const BwdPlan pl) {
+  using G = SGeo<F32, HDP>;
+  using PR = Pair<F32, HDP>;
+  // fp32 heads of 256: Q, dO and dq do not fit the register file together; Q and dO are read again (from the caches) for every tile
+  constexpr bool REREAD = F32 && HDP > 192;
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 768);
+  int* rsh = (int*)(smem + PR::IMAGES + 768 + 96);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int logical = xcd_remap(blockIdx.x, gridDim.x), split = logical % pl.sq, t1 = logical / pl.sq;
+  const int qb = pl.nqb - 1 - t1 % pl.nqb, bh = t1 / pl.nqb, b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.Hk);
+  const char* qbase = (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * G::ESZ;
+  // this wave's matrix of the pair: K (waves 0, 1) or V
+  const char* xbase = wave < 2 ? (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * G::ESZ
+                               : (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * G::ESZ;
+  const unsigned xrb = (unsigned)(wave < 2 ? a.k_ss : a.v_ss) * G::ESZ;
+  const int* kdoc = DOC ? a.k_doc + (size_t)b * a.Sk : nullptr;
+  const SMod m = smod(a, head);
+  const int p0 = q_pos0(a, b), pfx = prefix_of(a, b);
+  const int w0 = qb * 128 + wave * 32, i = w0 + (lane & 31), ic = min(i, a.Sq - 1);
+  const int qd = DOC ? a.q_doc[(size_t)b * a.Sq + ic] : 0;
+  const bool live = i < a.Sq && qd >= 0, wave_live = w0 < a.Sq;
+  const QRow qr = q_row(a, p0, pfx, w0, i);
+  const int hi = key_end(a, p0, pfx, min(qb * 128 + 127, a.Sq - 1));
+  const int units = (hi + 63) / 64, u_lo = (int)((long long)units * split / pl.sq), u_hi = (int)((long long)units * (split + 1) / pl.sq);
+  HalfWalk<DOC> walk{{kdoc, u_hi, a.Sk, 0, 0, 0, {}, true, false}, -1, min(hi, u_hi * 64), true, false};
+  if (DOC) doc_range(qd, live, rsh, wave, lane, walk.w.dmin, walk.w.dmax);
+  walk.first(2 * u_lo, dsh, wave, lane);
+  const typename PR::Dma dma(wave & 1, lane, xrb, a.D);
+  int* kds = (int*)(smem + PR::IMAGES);    // [3 images][64] documents of the keys (32 used)
+  auto fetch = [&](int buf) {
+    // (keys behind the last are hidden by the row's limit, whatever document they show)
+    if (DOC && wave == 0) __builtin_amdgcn_global_load_lds(TF_GLB_PTR(kdoc + min(walk.s * 32 + (lane & 31), a.Sk - 1)), TF_LDS_PTR(kds + buf * 64), 4, 0, 0);
+    dma.issue(xbase, xrb, walk.s * 32, hi, a.D, DOC && walk.neg ? kdoc : nullptr, smem + buf * PR::BUF + (wave >> 1) * PR::HALF);
+  };
+  const long long row = (long long)bh * a.Sq + ic, orow = (((long long)b * a.Sq + ic) * a.H + head) * a.D;
+  const char* qrow = qbase + (long long)ic * a.q_ss * G::ESZ;
+  SFrag<F32> qf[REREAD ? 1 : G::KS], dof[REREAD ? 1 : G::KS];
+  const char* drow = (const char*)a.dout + ((long long)b * a.do_sb + (long long)ic * a.do_ss + (long long)head * a.do_sh) * G::ESZ;
+  float delta = 0.f;
+  {
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ++ks) {
+      const SFrag<F32> d = gfrag<F32>(drow, ks, h, a.D, live);
+      delta += frag_dot<F32>(d, gfrag<F32>((const char*)a.out + orow * G::ESZ, ks, h, a.D, live));
+      if (!F32 && a.out_lo != nullptr) delta += frag_dot<F32>(d, gfrag<F32>((const char*)a.out_lo + orow * G::ESZ, ks, h, a.D, live));
+      if constexpr (!REREAD) {
+        qf[ks] = gfrag<F32>(qrow, ks, h, a.D, live);
+        dof[ks] = d;
+      }
+      if (F32 && HDP > 128) asm volatile("" ::: "memory");        // (a few loads at a time: the rows of O are not to lie in registers as a whole)
+    }
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  auto qx = [&](auto I) { if constexpr (REREAD) return gfrag<F32>(qrow, I, h, a.D, live); else return qf[I]; };
+  auto dx = [&](auto I) { if constexpr (REREAD) return gfrag<F32>(drow, I, h, a.D, live); else return dof[I]; };
+  float lse = live ? a.lse[row] : INFINITY;
+  landed(lse);
+  landed(delta);
+  if constexpr (!REREAD) {
+#pragma unroll
+    for (int ks = 0; ks < G::KS; ++ks) { landed(qf[ks]); landed(dof[ks]); }
+  }
+  Coming cur{}, nxt{};
+  auto take = [&](int image) {            // the pair the walk stands at goes to `image`
+    if (walk.s < 0) return Coming{};
+    fetch(image);
+    return Coming{walk.s, walk.full};
+  };
+  auto go_on = [&](int image) {
+    if (walk.s < 0) return Coming{};
+    walk.next(dsh, wave, lane);
+    return take(image);
+  };
+  cur = take(0);
+  if (PR::NB == 3) nxt = go_on(1);
+  f32x16 dq[G::DB];
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
+  std::conditional_t<F32, double, float> dsl = 0;        // (distances up to the length times small terms of both signs)
+  const SAddr<F32, HDP> fk0(lds_addr_of(smem), lane);
+  int buf = 0;
+  while (cur.s >= 0) {
+    const int kv0 = cur.s * 32;
+    const bool full_t = cur.full && kv0 + 31 <= qr.lim_lo, work = wave_live && kv0 <= qr.lim_hi;
+    PR::wait(nxt.s >= 0);
+    const Coming young = go_on(PR::NB == 3 ? PR::after(PR::after(buf)) : buf ^ 1);
+    if (work) {
+      const SAddr<F32, HDP> fk = fk0.shifted(buf * PR::BUF);
+      f32x16 st, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = 0.f; }
+      mul_rows2<F32, HDP, PR::HALF>(fk, qx, dx, st, dp);
+      unsigned bits = 0xffffffffu;
+      if (!full_t) {
+        bits = low_bits(qr.lim - kv0 + 1);
+        if (DOC) {
+          unsigned kd = rd32_asm<0>(lds_addr_of(kds + buf * 64) + (lane & 31) * 4);
+          lgkm_wait32<0>(kd);
+          bits &= (unsigned)doc_bits(qd, (int)kd);
+        }
+        bits >>= 4 * h;
+      }
+      const float pd = (float)(qr.p - kv0 - 4 * h), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
+      SPack<F32> pk[1];
+      const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
+      const int cap = m.capl == 0.f ? 0 : all_small<F32, 1>(m, raw) ? 2 : 1;
+      by_flags(full_t, cap, m.slope2 != 0.f || a.dslopes != nullptr, [&](auto FULL, auto CAP, auto SLP) {
+        auto one = [&](int r) {
+          const int j = (r & 3) + 8 * (r >> 2);
+          float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? capped_exact<F32>(m, st[r]) : st[r] * m.sc, x = t;
+          const float dist = SLP ? fabsf(pd - (float)j) : 0.f;
+          if (SLP) x -= m.slope2 * dist;
+          x = fast_exp2(x - lse) * (dp[r] - delta);
+          if (!FULL) x = (bits >> j) & 1u ? x : 0.f;
+          if (SLP) dsl -= x * dist;
+          return CAP ? x * fmaf(t * t, ncap, 1.0f) : x;           // the cap's derivative: 1 - (t / cap)^2
+        };
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float x0 = one(r), x1 = one(r + 1);
+          pk[0].set2(r, x0, x1);
+        }
+      });
+      fk.template mul_t<0>(pk, dq);
+    }
+    cur = PR::NB == 3 ? nxt : young;
+    nxt = young;
+    buf = PR::after(buf);
+  }
+  dsl += __shfl_xor(dsl, 32, 64);
+  const long long rows = (long long)a.B * a.H * a.Sq;
+  if (i < a.Sq && h == 0) {
+    if (split == 0) a.delta[row] = delta;
+    if (a.dslopes != nullptr) ((float*)a.work)[pl.o_rows + split * rows + row] = live ? (float)dsl : 0.f;
+  }
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[d][r] = live ? dq[d][r] : 0.f;
+  store_grad<F32, G::DB>(a.dq, (float*)a.work, rows * a.D, split, pl.sq, orow, dq, a.scale, h, a.D, i < a.Sq);
+}
+
+// ================================================================================================
+// dk, dv: key on the lane, 128 keys a workgroup, over the heads that share them and their queries.  PART 0: dv, 1: dk, 2: both
+// ================================================================================================
+template <bool F32, int HDP, int PART, bool DOC>
+__global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1 ? 128 : 192) ? 2 : 1)) void score_dkv_kernel(const TfScoreAttnArgs a, const BwdPlan pl) {
+  using G = SGeo<F32, HDP>;
+  using PR = Pair<F32, HDP>;
+  constexpr bool DK = PART != 0, DV = PART != 1;
+  constexpr bool REREAD = F32 && HDP > 192;              // as in score_dq_kernel: V is read again for every tile
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  float* stat = (float*)(smem + PR::IMAGES);             // [3 images][32 lse, 32 delta]
+  int* qds = (int*)(smem + PR::IMAGES + 768);             // [3 images][64] documents of the queries (32 used)
+  u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 1536);
+  int* rsh = (int*)(smem + PR::IMAGES + 1536 + 96);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int nsplit = pl.sg * pl.sk, logical = xcd_remap(blockIdx.x, gridDim.x), split = logical % nsplit, t1 = logical / nsplit;
+  const int kb = t1 % pl.nkb, bk = t1 / pl.nkb, b = bk / a.Hk, kvh = bk % a.Hk, G_ = a.H / a.Hk;
+  const char* kbase = (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * G::ESZ;
+  const char* vbase = (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * G::ESZ;
+  const int* qdoc = DOC ? a.q_doc + (size_t)b * a.Sq : nullptr;
+  const int p0 = q_pos0(a, b), pfx = prefix_of(a, b);
+  const int k0 = kb * 128, w0 = k0 + wave * 32, j = w0 + (lane & 31), jc = min(j, a.Sk - 1);
+  const int kd = DOC ? a.k_doc[(size_t)b * a.Sk + jc] : 0;
+  const bool live = j < a.Sk && kd >= 0, wave_live = w0 < a.Sk;
+  const char* vrow = vbase + (long long)jc * a.v_ss * G::ESZ;
+  SFrag<F32> kf[G::KS], vf[DK && !REREAD ? G::KS : 1];
+  // (keys no query sees may hold anything)
+  const bool seen = live && (!a.causal || j < pfx || j <= p0 + a.Sq - 1);
+#pragma unroll
+  for (int ks = 0; ks < G::KS; ++ks) {
+    kf[ks] = gfrag<F32>(kbase + (long long)jc * a.k_ss * G::ESZ, ks, h, a.D, seen);
+    if constexpr (DK && !REREAD) vf[ks] = gfrag<F32>(vrow, ks, h, a.D, seen);
+  }
+#pragma unroll
+  for (int ks = 0; ks < G::KS; ++ks) {
+    landed(kf[ks]);
+    if constexpr (DK && !REREAD) landed(vf[ks]);
+  }
+  auto kx = [&](auto I) { return kf[I]; };
+  auto vx = [&](auto I) { if constexpr (REREAD) return gfrag<F32>(vrow, I, h, a.D, seen); else return vf[I]; };
+  f32x16 dk[DK ? G::DB : 1], dv[DV ? G::DB : 1];
+#pragma unroll
+  for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      if constexpr (DK) dk[d][r] = 0.f;
+      if constexpr (DV) dv[d][r] = 0.f;
+    }
+  // queries from q_lane on see this lane's key; the block's first key is seen from i_lo on, the wave's last key by all from q_full on
+  const int q_lane = a.causal && j >= pfx ? j - p0 : -(1 << 30);
+  const int i_lo = a.causal && k0 >= pfx ? min(max(k0 - p0, 0), a.Sq) : 0;
+  const int w_last = min(w0 + 31, a.Sk - 1);
+  const int q_full = a.causal && w_last >= pfx ? w_last - p0 : -(1 << 30), q_any = a.causal && w0 >= pfx ? w0 - p0 : -(1 << 30);
+  const int s_g = split / pl.sk, s_k = split % pl.sk, g_lo = G_ * s_g / pl.sg, g_hi = G_ * (s_g + 1) / pl.sg;
+  const int u0 = i_lo / 64, units = (a.Sq + 63) / 64 - u0;
+  const int u_lo = u0 + (int)((long long)units * s_k / pl.sk), u_hi = u0 + (int)((long long)units * (s_k + 1) / pl.sk);
+  HalfWalk<DOC> walk{{qdoc, u_hi, a.Sq, 0, 0, 0, {}, true, false}, -1, min(a.Sq, u_hi * 64), true, false};
+  if (DOC) doc_range(kd, live, rsh, wave, lane, walk.w.dmin, walk.w.dmax);
+  const unsigned xrb = (unsigned)(wave < 2 ? a.q_ss : a.do_ss) * G::ESZ;
+  const typename PR::Dma dma(wave & 1, lane, xrb, a.D);
+  const SAddr<F32, HDP> fq0(lds_addr_of(smem), lane);
+  const unsigned stat0 = lds_addr_of(stat) + 16 * h;
+  for (int g = g_lo; g < g_hi; ++g) {
+    const int head = kvh * G_ + g;
+    const SMod m = smod(a, head);
+    const char* xbase = wave < 2 ? (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * G::ESZ
+                                 : (const char*)a.dout + ((long long)b * a.do_sb + (long long)head * a.do_sh) * G::ESZ;
+    const long long row0 = ((long long)b * a.H + head) * a.Sq;
+    auto fetch = [&](int buf) {           // the pair in walk.s, its rows' statistics (wave 0: 32 of each, 4 bytes a lane) and documents
+      const int i0 = walk.s * 32;
+      // (queries behind the last are hidden by number, whatever document they show)
+      if (DOC && wave == 1) __builtin_amdgcn_global_load_lds(TF_GLB_PTR(qdoc + min(i0 + (lane & 31), a.Sq - 1)), TF_LDS_PTR(qds + buf * 64), 4, 0, 0);
+      if (wave == 0) {
+        const float* src = (lane < 32 ? a.lse : a.delta) + row0 + min(i0 + (lane & 31), a.Sq - 1);
+        __builtin_amdgcn_global_load_lds(TF_GLB_PTR(src), TF_LDS_PTR(stat + buf * 64), 4, 0, 0);
+      }
+      dma.issue(xbase, xrb, i0, a.Sq, a.D, DOC && walk.neg ? qdoc : nullptr, smem + buf * PR::BUF + (wave >> 1) * PR::HALF);
+    };
+    Coming cur{}, nxt{};
+    auto take = [&](int image) {
+      if (walk.s < 0) return Coming{};
+      fetch(image);
+      return Coming{walk.s, walk.full};
+    };
+    auto go_on = [&](int image) {
+      if (walk.s < 0) return Coming{};
+      walk.next(dsh, wave, lane);
+      return take(image);
+    };
+    walk.first(max(i_lo / 32, 2 * u_lo), dsh, wave, lane);
+    if (g > g_lo) __syncthreads();        // every wave is done with the images of the head before
+    int buf = 0;
+    cur = take(0);
+    if (PR::NB == 3) nxt = go_on(1);
+    while (cur.s >= 0) {
+      const int i0 = cur.s * 32;
+      const bool full_t = cur.full && i0 >= q_full && i0 + 32 <= a.Sq, work = wave_live && i0 + 31 >= q_any;
+      PR::wait(nxt.s >= 0);
+      const Coming young = go_on(PR::NB == 3 ? PR::after(PR::after(buf)) : buf ^ 1);
+      if (work) {
+        const SAddr<F32, HDP> fq = fq0.shifted(buf * PR::BUF);
+        f32x16 st, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[r] = 0.f;
+        u32x4 ls[4];                      // register 4 g + e is query 8 g + 4 h + e
+        const unsigned sa = stat0 + buf * 256;
+        static_for<4>([&](auto I) { ls[I] = rd128_asm<32 * I>(sa); });
+        if constexpr (DK) {               // dP - delta: the product starts at -delta
+          u32x4 de[4];
+          static_for<4>([&](auto I) { de[I] = rd128_asm<128 + 32 * I>(sa); });
+          static_for<4>([&](auto I) {
+            lgkm_wait<0>(de[I]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[4 * I + e] = -f_of(de[I][e]);
+          });
+          mul_rows2<F32, HDP, PR::HALF>(fq, kx, vx, st, dp);
+        } else mul_rows<F32, HDP>(fq, kx, st);
+        unsigned bits = 0xffffffffu;
+        if (!full_t) {
+          bits = ~low_bits(max(q_lane - i0, 0)) & low_bits(a.Sq - i0);
+          if (DOC) {
+            unsigned qd = rd32_asm<0>(lds_addr_of(qds + buf * 64) + (lane & 31) * 4);
+            lgkm_wait32<0>(qd);
+            bits &= (unsigned)doc_bits(kd, (int)qd);
+          }
+          bits >>= 4 * h;
+        }
+        static_for<4>([&](auto I) { lgkm_wait<0>(ls[I]); });
+        const float pd = (float)(p0 + i0 + 4 * h - j), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
+        SPack<F32> pp[1], ps[1];
+        const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
+        const int cap = m.capl == 0.f ? 0 : all_small<F32, 1>(m, raw) ? 2 : 1;
+        by_flags(full_t, cap, m.slope2 != 0.f, [&](auto FULL, auto CAP, auto SLP) {
+          auto one = [&](int r, float& pr, float& ds) {
+            const int q = (r & 3) + 8 * (r >> 2);
+            float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? capped_exact<F32>(m, st[r]) : st[r] * m.sc, x = t;
+            if (SLP) x -= m.slope2 * fabsf(pd + (float)q);
+            pr = fast_exp2(x - f_of(ls[r >> 2][r & 3]));
+            if (!FULL) pr = (bits >> q) & 1u ? pr : 0.f;
+            if constexpr (DK) {
+              ds = pr * dp[r];
+              if (CAP) ds *= fmaf(t * t, ncap, 1.0f);
+              if (!FULL) ds = (bits >> q) & 1u ? ds : 0.f;        // (a hidden pair's product may not be finite)
+            }
+          };
+#pragma unroll
+          for (int r = 0; r < 16; r += 2) {
+            float p0_, p1_, s0_ = 0.f, s1_ = 0.f;
+            one(r, p0_, s0_);
+            one(r + 1, p1_, s1_);
+            if constexpr (DV) pp[0].set2(r, p0_, p1_);
+            if constexpr (DK) ps[0].set2(r, s0_, s1_);
+          }
+        });
+        if constexpr (DV) fq.template mul_t<PR::HALF>(pp, dv);
+        if constexpr (DK) fq.template mul_t<0>(ps, dk);
+      }
+      cur = PR::NB == 3 ? nxt : young;
+      nxt = young;
+      buf = PR::after(buf);
+    }
+  }
+  const long long go = (((long long)b * a.Sk + jc) * a.Hk + kvh) * a.D, n = (long long)a.B * a.Sk * a.Hk * a.D;
+  if constexpr (DK) {
+#pragma unroll
+    for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dk[d][r] = live ? dk[d][r] : 0.f;
+    store_grad<F32, G::DB>(a.dk, (float*)a.work + pl.o_dk, n, split, nsplit, go, dk, a.scale, h, a.D, j < a.Sk);
+  }
+  if constexpr (DV) {
+#pragma unroll
+    for (int d = 0; d < G::DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dv[d][r] = live ? dv[d][r] : 0.f;
+    store_grad<F32, G::DB>(a.dv, (float*)a.work + pl.o_dv, n, split, nsplit, go, dv, 1.0f, h, a.D, j < a.Sk);
+  }
+}
+
+// out = scale * (part 0 + part 1 + ...), rounded once
+template <bool F32> __global__ __launch_bounds__(256) void score_sum_kernel(const float* __restrict__ parts, long long n, int nsplit, float scale, void* out) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  f32x4 s = *(const f32x4*)(parts + i);
+#pragma unroll 4
+  for (int k = 1; k < nsplit; ++k) s += *(const f32x4*)(parts + (long long)k * n + i);
+  put4<F32>(out, i, s[0] * scale, s[1] * scale, s[2] * scale, s[3] * scale);
+}
+
+// the slopes' gradient: one workgroup a head adds up the rows of all samples (and parts: B counts those), in 64 bits and in one order
+__global__ __launch_bounds__(256) void score_dslope_kernel(const float* __restrict__ rows, float* __restrict__ out, int B, int H, int Sq) {
+  __shared__ double sh[256];
+  const int head = blockIdx.x, tid = threadIdx.x;
+  double s = 0.0;
+  for (int b = 0; b < B; ++b) {
+    const float* r = rows + ((size_t)b * H + head) * Sq;
+    for (int i = tid; i < Sq; i += 256) s += (double)r[i];
+  }
+  sh[tid] = s;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (tid < o) sh[tid] += sh[tid + o];
+    __syncthreads();
+  }
+  if (tid == 0) out[head] = (float)sh[0];
+}
+
+// ================================================================================================
+// launchers
+// ================================================================================================
+BwdPlan bwd_plan(const TfScoreAttnArgs* a, bool slopes) {
+  BwdPlan p;
+  const int G = a->H / a->Hk;
+  p.nqb = (a->Sq + 127) / 128;
+  p.nkb = (a->Sk + 127) / 128;
+  // Too few workgroups for 256 CUs: the loops are split until two a CU are there, each with at least four to eight pairs of tiles.  dk / dv are split
+  // by heads first (each is a loop of its own), and up to four a CU: with shared heads a workgroup's loop is long and uneven.
+  const long long bq = (long long)a->B * a->H * p.nqb, bk = (long long)a->B * a->Hk * p.nkb;
+  auto ways = [](long long blocks, long long target, long long most) { return (int)std::max(1ll, std::min(blocks >= target / 2 ? 1 : (target + blocks - 1) / blocks, most)); };
+  p.sq = bq == 0 ? 1 : ways(bq, 512, (a->Sk + 127) / 128);
+  p.sg = bk == 0 ? 1 : (int)std::max(1ll, std::min({(1024 + bk - 1) / bk, (long long)G, (long long)G * ((a->Sq + 31) / 32) / 8}));
+  p.sk = bk == 0 ? 1 : ways(bk * p.sg, 512, (a->Sq + 127) / 128);
+  const size_t nq = (size_t)a->B * a->Sq * a->H * a->D, nk = (size_t)a->B * a->Sk * a->Hk * a->D, ns = (size_t)p.sg * p.sk;
+  p.o_dk = p.sq > 1 ? p.sq * nq : 0;
+  p.o_dv = p.o_dk + (ns > 1 ? ns * nk : 0);
+  p.o_rows = p.o_dv + (ns > 1 ? ns * nk : 0);
+  p.floats = p.o_rows + (slopes ? (size_t)p.sq * a->B * a->H * a->Sq : 0);
+  return p;
+}
+
+template <bool F32> void launch_sum(const TfScoreAttnArgs* a, size_t off, long long n, int nsplit, float scale, void* out, hipStream_t st) {
+  TfTraceScope tr("score_sum_kernel", st);
+  hipLaunchKernelGGL(score_sum_kernel<F32>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, (const float*)a->work + off, n, nsplit, scale, out);
+}
+
+template <bool F32, int HDP> int launch_bwd(const TfScoreAttnArgs* a, hipStream_t st) {
+  const double fl = 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D;
+  const BwdPlan pl = bwd_plan(a, a->dslopes != nullptr);
+  const bool doc = a->k_doc != nullptr;
+  const size_t lds = Pair<F32, HDP>::IMAGES + 1536 + 128;
+  auto go = [&](auto kern, int blocks) {
+    allow_lds(kern, lds);
+    hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), lds, st, *a, pl);
+  };
+  if (pl.nqb > 0) {
+    {
+      TfTraceScope tr(F32 ? "score_dq_kernel<fp32>" : "score_dq_kernel<bf16>", st, 1.5 * fl);
+      const int blocks = a->B * a->H * pl.nqb * pl.sq;
+      doc ? go(score_dq_kernel<F32, HDP, true>, blocks) : go(score_dq_kernel<F32, HDP, false>, blocks);
+    }
+    if (pl.sq > 1) launch_sum<F32>(a, 0, (long long)a->B * a->Sq * a->H * a->D, pl.sq, a->scale, a->dq, st);
+  }
+  if (a->dslopes != nullptr) {
+    TfTraceScope tr("score_dslope_kernel", st);
+    hipLaunchKernelGGL(score_dslope_kernel, dim3(a->H), dim3(256), 0, st, (const float*)a->work + pl.o_rows, a->dslopes, a->B * pl.sq, a->H, a->Sq);
+  }
+  if (pl.nkb > 0) {
+    {
+      TfTraceScope tr(F32 ? "score_dkv_kernel<fp32>" : "score_dkv_kernel<bf16>", st, 2.0 * fl);
+      const int blocks = a->B * a->Hk * pl.nkb * pl.sg * pl.sk;
+      auto part = [&](auto which) {
+        constexpr int PART = decltype(which)::value;
+        doc ? go(score_dkv_kernel<F32, HDP, PART, true>, blocks) : go(score_dkv_kernel<F32, HDP, PART, false>, blocks);
+      };
+      if constexpr (HDP <= (F32 ? 128 : 192)) part(std::integral_constant<int, 2>{});
+      else { part(std::integral_constant<int, 0>{}); part(std::integral_constant<int, 1>{}); }
+    }
+    const int ns = pl.sg * pl.sk;
+    const long long n = (long long)a->B * a->Sk * a->Hk * a->D;
+    if (ns > 1) {
+      launch_sum<F32>(a, pl.o_dk, n, ns, a->scale, a->dk, st);
+      launch_sum<F32>(a, pl.o_dv, n, ns, 1.0f, a->dv, st);
+    }
+  }
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+// bytes of TfScoreAttnArgs.work for the backward
+extern "C" size_t tf_score_attn_bwd_work(int B, int Sq, int Sk, int H, int Hk, int D, int is_f32, int slopes) {
+  TfScoreAttnArgs a{};
+  a.B = B; a.Sq = Sq; a.Sk = Sk; a.H = H; a.Hk = Hk; a.D = D; a.is_f32 = is_f32;
+  return score_check(&a) != 0 ? 0 : bwd_plan(&a, slopes != 0).floats * sizeof(float);
+}
+
+extern "C" int tf_launch_score_bwd(const TfScoreAttnArgs* a, hipStream_t st) {
+  const int rc = score_check(a);
+  if (rc != 0) return rc;
+  const int e = a->is_f32 ? 4 : 2;
+  if (a->B > 0 && a->Sq > 0 && (a->q == nullptr || a->out == nullptr || a->dout == nullptr || a->dq == nullptr || a->lse == nullptr || a->delta == nullptr)) return -6;
+  if (a->B > 0 && a->Sk > 0 && (a->k == nullptr || a->v == nullptr || a->dk == nullptr || a->dv == nullptr)) return -6;
+  if (a->dslopes != nullptr && a->slopes == nullptr) return -6;
+  if (!score_aligned(a->q, a->q_sb, a->q_ss, a->q_sh, e) || !score_aligned(a->k, a->k_sb, a->k_ss, a->k_sh, e) || !score_aligned(a->v, a->v_sb, a->v_ss, a->v_sh, e) ||
+      !score_aligned(a->dout, a->do_sb, a->do_ss, a->do_sh, e) || !score_aligned(a->out, 0, 0, 0, e) || !score_aligned(a->out_lo, 0, 0, 0, e) ||
+      !score_aligned(a->dq, 0, 0, 0, e) || !score_aligned(a->dk, 0, 0, 0, e) || !score_aligned(a->dv, 0, 0, 0, e)) return -7;
+  const size_t need = bwd_plan(a, a->dslopes != nullptr).floats * sizeof(float);
+  if (need > 0 && (a->work == nullptr || a->work_bytes < need || ((uintptr_t)a->work & 15) != 0)) return -8;
+  if (a->B == 0) {
+    if (a->dslopes != nullptr) hipLaunchKernelGGL(score_dslope_kernel, dim3(a->H), dim3(256), 0, st, (const float*)nullptr, a->dslopes, 0, a->H, 0);
+    return (int)hipGetLastError();
+  }
+  return by_head_dim(a, [&](auto f32, auto hdp) { return launch_bwd<decltype(f32)::value, decltype(hdp)::value>(a, st); });
+}

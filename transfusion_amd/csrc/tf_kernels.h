@@ -59,7 +59,7 @@ int tf_launch_im2col(const TfPatchArgs* a, hipStream_t stream);       // feat ->
 int tf_launch_col2im(const TfPatchArgs* a, int out_is_f32, hipStream_t stream);  // cols -> feat (fold; border zero)
 int tf_launch_split_planes(const TfPlanesArgs* a, hipStream_t st);
 int tf_launch_rotary(const TfRotaryArgs* a, hipStream_t st);            // rotary.hip
-int tf_launch_score_fwd(const TfScoreAttnArgs* a, hipStream_t st);      // score_attn.hip
+int tf_launch_score_fwd(const TfScoreAttnArgs* a, hipStream_t st);      // score_attn_fwd.hip
 int tf_launch_score_bwd(const TfScoreAttnArgs* a, hipStream_t st);
 int tf_launch_grad_clip(const TfGradClipArgs* a, hipStream_t st);       // gradnorm.hip
 
