@@ -7,18 +7,12 @@
 
 namespace {
 
-// Two 32-row tiles that are used together (K and V, or Q and dO) as one image: waves 0 and 1 fetch the first, 2 and 3 the second.  Three
-// images: two pairs are under way while one is worked on, one barrier a pair; a wave waits for its own transfers of the older pair by
-// count (a pair is NI of them, everything else it issues in between only makes the wait longer).  fp32 heads of 256 have room for two.
+// Two 32-row tiles that are used together (K and V, or Q and dO) as one image: waves 0 and 1 fetch the first, 2 and 3 the second.  Two
+// images, one barrier a pair: the next pair is under way while one is worked on.  (A third image, transfers waited for by count, gained
+// nothing: 4 x 4096 causal, 8 heads of 128, 653 against 603 us, and 4 x 2048, 16 heads of 64, 308 either way.)
 template <bool F32, int HDP> struct Pair {
   using Dma = SDma<F32, HDP, 32, 2>;
-  static constexpr int HALF = Dma::BYTES, BUF = 2 * HALF, NB = F32 && HDP > 192 ? 2 : 3, IMAGES = NB * BUF;
-  // the pair in hand is there (younger, with three images: another one is under way behind it), and every wave is done with the one before
-  static __device__ __forceinline__ void wait(bool younger) {
-    if (NB == 3 && younger) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(Dma::NI) : "memory");
-    else dma_wait_barrier();
-  }
-  static __device__ __forceinline__ int after(int image) { return image + 1 == NB ? 0 : image + 1; }
+  static constexpr int HALF = Dma::BYTES, BUF = 2 * HALF, IMAGES = 2 * BUF;
 };
 
 // a pair under way: half-tile number (-1: none), full (see TileWalk)
@@ -47,11 +41,11 @@ template <bool F32, int HDP, bool DOC>
 __global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_dq_kernel(const TfScoreAttnArgs a, const BwdPlan pl) {
   using G = SGeo<F32, HDP>;
   using PR = Pair<F32, HDP>;
-  // fp32 heads of 256: Q, dO and dq do not fit the register file together; Q and dO are read again (from the caches) for every tile
-  constexpr bool REREAD = F32 && HDP > 192;
+  // fp32 heads of 256 (of 192 with documents): Q, dO and dq do not fit the register file together; Q and dO are read again (from the caches) for every tile
+  constexpr bool REREAD = F32 && (HDP > 192 || (HDP > 128 && DOC));
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 768);
-  int* rsh = (int*)(smem + PR::IMAGES + 768 + 96);
+  u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 512);
+  int* rsh = (int*)(smem + PR::IMAGES + 512 + 96);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int logical = xcd_remap(blockIdx.x, gridDim.x), split = logical % pl.sq, t1 = logical / pl.sq;
   const int qb = pl.nqb - 1 - t1 % pl.nqb, bh = t1 / pl.nqb, b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.Hk);
@@ -73,7 +67,7 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_
   if (DOC) doc_range(qd, live, rsh, wave, lane, walk.w.dmin, walk.w.dmax);
   walk.first(2 * u_lo, dsh, wave, lane);
   const typename PR::Dma dma(wave & 1, lane, xrb, a.D);
-  int* kds = (int*)(smem + PR::IMAGES);    // [3 images][64] documents of the keys (32 used)
+  int* kds = (int*)(smem + PR::IMAGES);    // [2 images][64] documents of the keys (32 used)
   auto fetch = [&](int buf) {
     // (keys behind the last are hidden by the row's limit, whatever document they show)
     if (DOC && wave == 0) __builtin_amdgcn_global_load_lds(TF_GLB_PTR(kdoc + min(walk.s * 32 + (lane & 31), a.Sk - 1)), TF_LDS_PTR(kds + buf * 64), 4, 0, 0);
@@ -107,7 +101,7 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_
 #pragma unroll
     for (int ks = 0; ks < G::KS; ++ks) { landed(qf[ks]); landed(dof[ks]); }
   }
-  Coming cur{}, nxt{};
+  Coming cur{};
   auto take = [&](int image) {            // the pair the walk stands at goes to `image`
     if (walk.s < 0) return Coming{};
     fetch(image);
@@ -119,7 +113,6 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_
     return take(image);
   };
   cur = take(0);
-  if (PR::NB == 3) nxt = go_on(1);
   f32x16 dq[G::DB];
 #pragma unroll
   for (int d = 0; d < G::DB; ++d)
@@ -131,8 +124,8 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_
   while (cur.s >= 0) {
     const int kv0 = cur.s * 32;
     const bool full_t = cur.full && kv0 + 31 <= qr.lim_lo, work = wave_live && kv0 <= qr.lim_hi;
-    PR::wait(nxt.s >= 0);
-    const Coming young = go_on(PR::NB == 3 ? PR::after(PR::after(buf)) : buf ^ 1);
+    dma_wait_barrier();                  // the pair in hand is there, and every wave is done with the one before
+    const Coming nxt = go_on(buf ^ 1);
     if (work) {
       const SAddr<F32, HDP> fk = fk0.shifted(buf * PR::BUF);
       f32x16 st, dp;
@@ -172,9 +165,8 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_
       });
       fk.template mul_t<0>(pk, dq);
     }
-    cur = PR::NB == 3 ? nxt : young;
-    nxt = young;
-    buf = PR::after(buf);
+    cur = nxt;
+    buf ^= 1;
   }
   dsl += __shfl_xor(dsl, 32, 64);
   const long long rows = (long long)a.B * a.H * a.Sq;
@@ -199,10 +191,10 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1
   constexpr bool DK = PART != 0, DV = PART != 1;
   constexpr bool REREAD = F32 && HDP > 192;              // as in score_dq_kernel: V is read again for every tile
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  float* stat = (float*)(smem + PR::IMAGES);             // [3 images][32 lse, 32 delta]
-  int* qds = (int*)(smem + PR::IMAGES + 768);             // [3 images][64] documents of the queries (32 used)
-  u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 1536);
-  int* rsh = (int*)(smem + PR::IMAGES + 1536 + 96);
+  float* stat = (float*)(smem + PR::IMAGES);             // [2 images][32 lse, 32 delta]
+  int* qds = (int*)(smem + PR::IMAGES + 512);             // [2 images][64] documents of the queries (32 used)
+  u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 1024);
+  int* rsh = (int*)(smem + PR::IMAGES + 1024 + 96);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int nsplit = pl.sg * pl.sk, logical = xcd_remap(blockIdx.x, gridDim.x), split = logical % nsplit, t1 = logical / nsplit;
   const int kb = t1 % pl.nkb, bk = t1 / pl.nkb, b = bk / a.Hk, kvh = bk % a.Hk, G_ = a.H / a.Hk;
@@ -267,7 +259,7 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1
       }
       dma.issue(xbase, xrb, i0, a.Sq, a.D, DOC && walk.neg ? qdoc : nullptr, smem + buf * PR::BUF + (wave >> 1) * PR::HALF);
     };
-    Coming cur{}, nxt{};
+    Coming cur{};
     auto take = [&](int image) {
       if (walk.s < 0) return Coming{};
       fetch(image);
@@ -282,12 +274,11 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1
     if (g > g_lo) __syncthreads();        // every wave is done with the images of the head before
     int buf = 0;
     cur = take(0);
-    if (PR::NB == 3) nxt = go_on(1);
     while (cur.s >= 0) {
       const int i0 = cur.s * 32;
       const bool full_t = cur.full && i0 >= q_full && i0 + 32 <= a.Sq, work = wave_live && i0 + 31 >= q_any;
-      PR::wait(nxt.s >= 0);
-      const Coming young = go_on(PR::NB == 3 ? PR::after(PR::after(buf)) : buf ^ 1);
+      dma_wait_barrier();                  // the pair in hand is there, and every wave is done with the one before
+      const Coming nxt = go_on(buf ^ 1);
       if (work) {
         const SAddr<F32, HDP> fq = fq0.shifted(buf * PR::BUF);
         f32x16 st, dp;
@@ -346,9 +337,8 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1
         if constexpr (DV) fq.template mul_t<PR::HALF>(pp, dv);
         if constexpr (DK) fq.template mul_t<0>(ps, dk);
       }
-      cur = PR::NB == 3 ? nxt : young;
-      nxt = young;
-      buf = PR::after(buf);
+      cur = nxt;
+      buf ^= 1;
     }
   }
   const long long go = (((long long)b * a.Sk + jc) * a.Hk + kvh) * a.D, n = (long long)a.B * a.Sk * a.Hk * a.D;
@@ -428,7 +418,7 @@ template <bool F32, int HDP> int launch_bwd(const TfScoreAttnArgs* a, hipStream_
   const double fl = 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D;
   const BwdPlan pl = bwd_plan(a, a->dslopes != nullptr);
   const bool doc = a->k_doc != nullptr;
-  const size_t lds = Pair<F32, HDP>::IMAGES + 1536 + 128;
+  const size_t lds = Pair<F32, HDP>::IMAGES + 1024 + 128;
   auto go = [&](auto kern, int blocks) {
     allow_lds(kern, lds);
     hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), lds, st, *a, pl);

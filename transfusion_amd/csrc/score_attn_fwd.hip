@@ -3,28 +3,18 @@
 
 namespace {
 
-// 128 queries a workgroup (32 a wave, on the lane), 64-key tiles by LDS-DMA into a ring of three slots, K(0) V(0) K(1) V(1) ...: K(t + 1) is
-// asked for before S(t), V(t + 1) before PV(t), so a transfer has a whole tile's work to travel under.  Where three slots would cost
-// a workgroup a CU (bf16 heads of 192: two workgroups of two slots) or do not fit, two: V(t) travels under S(t), K(t + 1) under PV(t).
-// Several workgroups a CU hide the barriers of one behind the matrix work of the others.  DOC: documents are given.
-template <bool F32, int HDP> struct FwdRing {
-  using Dma = SDma<F32, HDP, 64, 4>;
-  static constexpr int SLOTS = F32 ? (HDP > 192 ? 2 : 3) : (HDP > 128 && HDP <= 192 ? 2 : 3);
-  static __device__ __forceinline__ void wait(bool younger) {          // (younger: a transfer behind the wanted one is under way)
-    if (SLOTS == 3 && younger) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(Dma::NI) : "memory");
-    else dma_wait_barrier();
-  }
-  static __device__ __forceinline__ int after(int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; }
-};
+// 128 queries a workgroup (32 a wave, on the lane), 64-key tiles by LDS-DMA into one slot for K and one for V: V(t) travels under S(t), K(t + 1)
+// under PV(t).  Several workgroups a CU hide the barriers of one behind the matrix work of the others.  (A third slot, which gives a transfer a
+// whole tile's work to travel under, costs a workgroup a CU or gains nothing: 4 x 4096 causal, 8 heads of 128, 177 against 168 us; 4 x 2048, 16
+// heads of 64, 87 against 84.)  DOC: documents are given.
 template <bool F32, int HDP, bool DOC>
 __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <= 96 ? 3 : HDP <= (F32 ? 64 : 192) ? 2 : 1)) void score_fwd_kernel(const TfScoreAttnArgs a, int nqb, int nsplit, int split_tiles) {
   using G = SGeo<F32, HDP>;
-  using R = FwdRing<F32, HDP>;
-  using Dma = typename R::Dma;
+  using Dma = SDma<F32, HDP, 64, 4>;
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  u64 (*dsh)[3] = (u64 (*)[3])(smem + R::SLOTS * Dma::BYTES);
-  int* rsh = (int*)(smem + R::SLOTS * Dma::BYTES + 96);
-  int* kds = (int*)(smem + R::SLOTS * Dma::BYTES + 128);         // [2][64] documents of the keys of two tiles
+  u64 (*dsh)[3] = (u64 (*)[3])(smem + 2 * Dma::BYTES);
+  int* rsh = (int*)(smem + 2 * Dma::BYTES + 96);
+  int* kds = (int*)(smem + 2 * Dma::BYTES + 128);         // [2][64] documents of the keys of two tiles
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int logical = xcd_remap(blockIdx.x, gridDim.x);
   const int split = logical % nsplit, t1 = logical / nsplit;
@@ -64,22 +54,19 @@ __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <
   const Dma dma(wave, lane, krb, a.D);
   int t = walk.first(split * split_tiles, dsh, wave, lane);
   bool full = walk.full, neg = walk.neg;
-  int slot = 0, dslot = 0;                // of K(t), of its documents
-  auto issue_k = [&](int tile, bool ng, int to) {
+  int dslot = 0;                          // of the documents of K(t)
+  auto issue_k = [&](int tile, bool ng) {
     // (keys behind the last are hidden by the row's limit, whatever document they show)
     if (DOC && wave == 0) __builtin_amdgcn_global_load_lds(TF_GLB_PTR(kdoc + min(tile * 64 + lane, a.Sk - 1)), TF_LDS_PTR(kds + dslot * 64), 4, 0, 0);
     dslot ^= 1;
-    dma.issue(kbase, krb, tile * 64, hi, a.D, DOC && ng ? kdoc : nullptr, smem + to * Dma::BYTES);
+    dma.issue(kbase, krb, tile * 64, hi, a.D, DOC && ng ? kdoc : nullptr, smem);
   };
-  auto issue_v = [&](int tile, bool ng, int to) { dma.issue(vbase, vrb, tile * 64, hi, a.D, DOC && ng ? kdoc : nullptr, smem + to * Dma::BYTES); };
+  auto issue_v = [&](int tile, bool ng) { dma.issue(vbase, vrb, tile * 64, hi, a.D, DOC && ng ? kdoc : nullptr, smem + Dma::BYTES); };
   if constexpr (!REREAD) {
 #pragma unroll
     for (int ks = 0; ks < G::KS; ++ks) landed(qf[ks]);
   }
-  if (t >= 0) {
-    issue_k(t, neg, 0);
-    if (R::SLOTS == 3) issue_v(t, neg, 1);
-  }
+  if (t >= 0) issue_k(t, neg);
   while (t >= 0) {
     const int kv0 = t * 64;
     const bool full_t = full && kv0 + 63 <= row_.lim_lo, work = wave_live && kv0 <= row_.lim_hi;
@@ -88,10 +75,8 @@ __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <
     const bool neg_t = neg;
     full = walk.full;
     neg = walk.neg;
-    R::wait(true);                        // K(t) is there; every wave is done with V(t - 1)
-    if (R::SLOTS == 3) { if (tn >= 0) issue_k(tn, neg, R::after(R::after(slot))); }
-    else issue_v(t, neg_t, 1);
-    const SAddr<F32, HDP> fk = R::SLOTS == 2 ? f0 : f0.shifted(slot * Dma::BYTES);
+    dma_wait_barrier();                   // K(t) is there; every wave is done with V(t - 1)
+    issue_v(t, neg_t);
     SPack<F32> pk[2];
     if (work) {
       f32x16 st[2];
@@ -100,7 +85,7 @@ __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[kb][r] = 0.f;
       auto qx = [&](auto I) { if constexpr (REREAD) return gfrag<F32>(qrow, I, h, a.D, live); else return qf[I]; };
-      mul_rows2<F32, HDP, 32 * G::STR>(fk, qx, qx, st[0], st[1]);
+      mul_rows2<F32, HDP, 32 * G::STR>(f0, qx, qx, st[0], st[1]);
       // each change is a branch that rewrites the scores in place (uniform; as two arms of one branch they cost a second set of registers)
       if (m.capl != 0.f) {
         float c0 = m.c0, c1 = m.c1, c2 = m.c2, c3 = m.c3;
@@ -175,13 +160,12 @@ __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <
         }
       l_run += ps0 + ps1;
     }
-    R::wait(tn >= 0);                     // V(t) is there; every wave is done with K(t)
-    if (tn >= 0) { if (R::SLOTS == 3) issue_v(tn, neg, slot); else issue_k(tn, neg, 0); }
+    dma_wait_barrier();                   // V(t) is there; every wave is done with K(t)
+    if (tn >= 0) issue_k(tn, neg);
     if (work) {
-      if constexpr (R::SLOTS == 2 && !F32) f0.template mul_t<Dma::BYTES>(pk, o);
-      else f0.shifted(R::after(slot) * Dma::BYTES).template mul_t<0>(pk, o);
+      if constexpr (!F32) f0.template mul_t<Dma::BYTES>(pk, o);
+      else f0.shifted(Dma::BYTES).template mul_t<0>(pk, o);
     }
-    if (R::SLOTS == 3) slot = R::after(R::after(slot));
     t = tn;
   }
   const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
@@ -582,7 +566,7 @@ template <bool F32, int HDP> int launch_fwd(const TfScoreAttnArgs* a, hipStream_
   } else {
     TfTraceScope tr(F32 ? "score_fwd_kernel<fp32>" : "score_fwd_kernel<bf16>", st, fl);
     auto go = [&](auto kern) {
-      const size_t lds = FwdRing<F32, HDP>::SLOTS * SDma<F32, HDP, 64, 4>::BYTES + 640;
+      const size_t lds = 2 * SDma<F32, HDP, 64, 4>::BYTES + 640;
       allow_lds(kern, lds);
       hipLaunchKernelGGL(kern, dim3(a->B * a->H * f.nqb * f.nsplit), dim3(256), lds, st, *a, f.nqb, f.nsplit, f.split_tiles);
     };
