@@ -491,6 +491,21 @@ __device__ __forceinline__ void doc_range(int d, bool live, int* sh, int wave, i
   dmin = __builtin_amdgcn_readfirstlane(min(min(sh[0], sh[1]), min(sh[2], sh[3])));
   dmax = __builtin_amdgcn_readfirstlane(max(max(sh[4], sh[5]), max(sh[6], sh[7])));
 }
+// Which block of rows (0: the one that sees most) and which group this workgroup has; `per` consecutive groups share keys.  Where the blocks differ
+// in work (causal), the heaviest of ALL groups come first, so that the light ones fill up the end.  A chiplet keeps the groups that share
+// keys (workgroups are dealt to the 8 chiplets in turn) and, where they divide evenly, takes samples with stride 8, for the sake of ragged lengths.
+__device__ __forceinline__ void order_blocks(int nb, int per, bool uneven, int& block, int& group) {
+  const int n = gridDim.x / nb;
+  if (!uneven) {
+    const int l = xcd_remap(blockIdx.x, gridDim.x);
+    block = l % nb;
+    group = l / nb;
+    return;
+  }
+  const int g = blockIdx.x % n, y = g >> 3;
+  block = blockIdx.x / n;
+  group = n / per % 8 == 0 ? (8 * (y / per) + (g & 7)) * per + y % per : n % 8 == 0 ? (g & 7) * (n >> 3) + y : g;
+}
 // what a query row may see: everything below follows from these
 struct QRow { int p, lim, lim_lo, lim_hi; };       // position; last visible key of this row, of the wave's first row, of its last
 __device__ __forceinline__ QRow q_row(const TfScoreAttnArgs& a, int p0, int pfx, int w0, int i) {

@@ -47,8 +47,9 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_
   u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 512);
   int* rsh = (int*)(smem + PR::IMAGES + 512 + 96);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int logical = xcd_remap(blockIdx.x, gridDim.x), split = logical % pl.sq, t1 = logical / pl.sq;
-  const int qb = pl.nqb - 1 - t1 % pl.nqb, bh = t1 / pl.nqb, b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.Hk);
+  int block, group;
+  order_blocks(pl.nqb, a.H / a.Hk * pl.sq, a.causal, block, group);
+  const int qb = pl.nqb - 1 - block, split = group % pl.sq, bh = group / pl.sq, b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.Hk);
   const char* qbase = (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * G::ESZ;
   // this wave's matrix of the pair: K (waves 0, 1) or V
   const char* xbase = wave < 2 ? (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * G::ESZ
@@ -196,8 +197,10 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1
   u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 1024);
   int* rsh = (int*)(smem + PR::IMAGES + 1024 + 96);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int nsplit = pl.sg * pl.sk, logical = xcd_remap(blockIdx.x, gridDim.x), split = logical % nsplit, t1 = logical / nsplit;
-  const int kb = t1 % pl.nkb, bk = t1 / pl.nkb, b = bk / a.Hk, kvh = bk % a.Hk, G_ = a.H / a.Hk;
+  const int nsplit = pl.sg * pl.sk;
+  int kb, group;
+  order_blocks(pl.nkb, nsplit, a.causal, kb, group);
+  const int split = group % nsplit, bk = group / nsplit, b = bk / a.Hk, kvh = bk % a.Hk, G_ = a.H / a.Hk;
   const char* kbase = (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * G::ESZ;
   const char* vbase = (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * G::ESZ;
   const int* qdoc = DOC ? a.q_doc + (size_t)b * a.Sq : nullptr;

@@ -16,9 +16,9 @@ __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <
   int* rsh = (int*)(smem + 2 * Dma::BYTES + 96);
   int* kds = (int*)(smem + 2 * Dma::BYTES + 128);         // [2][64] documents of the keys of two tiles
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
-  const int logical = xcd_remap(blockIdx.x, gridDim.x);
-  const int split = logical % nsplit, t1 = logical / nsplit;
-  const int qb = nqb - 1 - t1 % nqb, bh = t1 / nqb, b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.Hk);
+  int block, group;
+  order_blocks(nqb, a.H / a.Hk * nsplit, a.causal, block, group);
+  const int qb = nqb - 1 - block, split = group % nsplit, bh = group / nsplit, b = bh / a.H, head = bh % a.H, kvh = head / (a.H / a.Hk);
   const char* qbase = (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * G::ESZ;
   const char* kbase = (const char*)a.k + ((long long)b * a.k_sb + (long long)kvh * a.k_sh) * G::ESZ;
   const char* vbase = (const char*)a.v + ((long long)b * a.v_sb + (long long)kvh * a.v_sh) * G::ESZ;
