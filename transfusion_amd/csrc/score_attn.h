@@ -544,6 +544,16 @@ template <class K> void allow_lds(K kern, size_t bytes) {
   done.fetch_or(1ull << dev, std::memory_order_relaxed);
 }
 
+// Ways to split the `units` (tiles of keys or queries) of a loop that `blocks` workgroups run.  bf16: until two workgroups a CU are there, `least` units
+// each.  fp32, where a unit is sixteen times the matrix work: down to one unit, as long as all workgroups run at once (two a CU up to 64 channels, then
+// one) and only if that shortens the longest loop.  2 x 355 x 417, 6 heads of 88, fp32 (36 workgroups): forward 54 -> 24 us with the join, dq 34 -> 26, dk / dv 38 -> 30.
+inline int split_ways(bool f32, int D, long long blocks, long long units, int least) {
+  if (blocks == 0 || units <= 1) return 1;
+  if (!f32) return (int)std::max(1ll, blocks >= 256 ? 1ll : std::min((512 + blocks - 1) / blocks, units / least));
+  const long long ways = std::max(1ll, std::min((D <= 64 ? 512 : 256) / blocks, units)), each = (units + ways - 1) / ways;
+  return (int)((units + each - 1) / each);
+}
+
 inline int score_check(const TfScoreAttnArgs* a) {
   if (a->B < 0 || a->Sq < 0 || a->Sk < 0 || a->H <= 0 || a->Hk <= 0 || a->H % a->Hk != 0) return -1;
   if (a->D <= 0 || a->D > 256 || a->D % 8 != 0) return -2;

@@ -18,7 +18,7 @@ template <bool F32, int HDP> struct Pair {
 // a pair under way: half-tile number (-1: none), full (see TileWalk)
 struct Coming { int s = -1; bool full = false; };
 
-// A workgroup's part of the rows: parts [nsplit] of fp32 in the layout of the result, added up by score_sum_kernel
+// A workgroup's part of the rows: parts [nsplit] of fp32 in the layout of the result, added up by score_finish_kernel
 template <bool F32, int DB> __device__ __forceinline__ void store_grad(void* out, float* parts, long long n, int split, int nsplit, long long off,
                                                                        const f32x16 (&x)[DB], float scale, int h, int D, bool ok) {
   if (nsplit > 1) {
@@ -63,10 +63,10 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_
   const bool live = i < a.Sq && qd >= 0, wave_live = w0 < a.Sq;
   const QRow qr = q_row(a, p0, pfx, w0, i);
   const int hi = key_end(a, p0, pfx, min(qb * 128 + 127, a.Sq - 1));
-  const int units = (hi + 63) / 64, u_lo = (int)((long long)units * split / pl.sq), u_hi = (int)((long long)units * (split + 1) / pl.sq);
-  HalfWalk<DOC> walk{{kdoc, u_hi, a.Sk, 0, 0, 0, {}, true, false}, -1, min(hi, u_hi * 64), true, false};
+  const int units = (hi + 31) / 32, u_lo = (int)((long long)units * split / pl.sq), u_hi = (int)((long long)units * (split + 1) / pl.sq);
+  HalfWalk<DOC> walk{{kdoc, (u_hi + 1) / 2, a.Sk, 0, 0, 0, {}, true, false}, -1, min(hi, u_hi * 32), true, false};
   if (DOC) doc_range(qd, live, rsh, wave, lane, walk.w.dmin, walk.w.dmax);
-  walk.first(2 * u_lo, dsh, wave, lane);
+  walk.first(u_lo, dsh, wave, lane);
   const typename PR::Dma dma(wave & 1, lane, xrb, a.D);
   int* kds = (int*)(smem + PR::IMAGES);    // [2 images][64] documents of the keys (32 used)
   auto fetch = [&](int buf) {
@@ -238,9 +238,9 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1
   const int w_last = min(w0 + 31, a.Sk - 1);
   const int q_full = a.causal && w_last >= pfx ? w_last - p0 : -(1 << 30), q_any = a.causal && w0 >= pfx ? w0 - p0 : -(1 << 30);
   const int s_g = split / pl.sk, s_k = split % pl.sk, g_lo = G_ * s_g / pl.sg, g_hi = G_ * (s_g + 1) / pl.sg;
-  const int u0 = i_lo / 64, units = (a.Sq + 63) / 64 - u0;
+  const int u0 = i_lo / 32, units = (a.Sq + 31) / 32 - u0;
   const int u_lo = u0 + (int)((long long)units * s_k / pl.sk), u_hi = u0 + (int)((long long)units * (s_k + 1) / pl.sk);
-  HalfWalk<DOC> walk{{qdoc, u_hi, a.Sq, 0, 0, 0, {}, true, false}, -1, min(a.Sq, u_hi * 64), true, false};
+  HalfWalk<DOC> walk{{qdoc, (u_hi + 1) / 2, a.Sq, 0, 0, 0, {}, true, false}, -1, min(a.Sq, u_hi * 32), true, false};
   if (DOC) doc_range(kd, live, rsh, wave, lane, walk.w.dmin, walk.w.dmax);
   const unsigned xrb = (unsigned)(wave < 2 ? a.q_ss : a.do_ss) * G::ESZ;
   const typename PR::Dma dma(wave & 1, lane, xrb, a.D);
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1
       walk.next(dsh, wave, lane);
       return take(image);
     };
-    walk.first(max(i_lo / 32, 2 * u_lo), dsh, wave, lane);
+    walk.first(u_lo, dsh, wave, lane);
     if (g > g_lo) __syncthreads();        // every wave is done with the images of the head before
     int buf = 0;
     cur = take(0);
@@ -361,32 +361,42 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1
   }
 }
 
-// out = scale * (part 0 + part 1 + ...), rounded once
-template <bool F32> __global__ __launch_bounds__(256) void score_sum_kernel(const float* __restrict__ parts, long long n, int nsplit, float scale, void* out) {
-  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
-  f32x4 s = *(const f32x4*)(parts + i);
-#pragma unroll 4
-  for (int k = 1; k < nsplit; ++k) s += *(const f32x4*)(parts + (long long)k * n + i);
-  put4<F32>(out, i, s[0] * scale, s[1] * scale, s[2] * scale, s[3] * scale);
-}
-
-// the slopes' gradient: one workgroup a head adds up the rows of all samples (and parts: B counts those), in 64 bits and in one order
-__global__ __launch_bounds__(256) void score_dslope_kernel(const float* __restrict__ rows, float* __restrict__ out, int B, int H, int Sq) {
-  __shared__ double sh[256];
-  const int head = blockIdx.x, tid = threadIdx.x;
-  double s = 0.0;
-  for (int b = 0; b < B; ++b) {
-    const float* r = rows + ((size_t)b * H + head) * Sq;
-    for (int i = tid; i < Sq; i += 256) s += (double)r[i];
-  }
-  sh[tid] = s;
-  __syncthreads();
-  for (int o = 128; o > 0; o >>= 1) {
-    if (tid < o) sh[tid] += sh[tid + o];
+// What is left when dq, dk and dv are there, in one launch: the sums of a split gradient's parts (out = scale * (part 0 + part 1 + ...), rounded once; 1024
+// values a workgroup) and, by the first H workgroups, the slopes' gradient: a head's row sums over all samples and parts, in 64 bits and one order.
+struct Finish {
+  struct Sum { const float* parts; void* out; long long n; int nsplit; unsigned blocks; float scale; } sum[3];
+  const float* rows;
+  float* dslopes;
+  unsigned heads, H, Sq, planes;         // heads: H, or 0 without slopes; planes: samples times parts, [planes][H][Sq]
+};
+template <bool F32> __global__ __launch_bounds__(256) void score_finish_kernel(const Finish f) {
+  const int tid = threadIdx.x;
+  unsigned block = blockIdx.x;
+  if (block < f.heads) {
+    __shared__ double sh[256];
+    double s = 0.0;
+    const unsigned n = f.planes * f.Sq;   // (fits: H * n row sums at 128 a workgroup)
+#pragma unroll 8
+    for (unsigned i = tid; i < n; i += 256) s += (double)f.rows[((size_t)(i / f.Sq) * f.H + block) * f.Sq + i % f.Sq];
+    sh[tid] = s;
     __syncthreads();
+    for (int o = 128; o > 0; o >>= 1) {
+      if (tid < o) sh[tid] += sh[tid + o];
+      __syncthreads();
+    }
+    if (tid == 0) f.dslopes[block] = (float)sh[0];
+    return;
   }
-  if (tid == 0) out[head] = (float)sh[0];
+  block -= f.heads;
+  int w = 0;
+  while (w < 2 && block >= f.sum[w].blocks) block -= f.sum[w++].blocks;
+  const Finish::Sum& u = f.sum[w];
+  const long long i = ((long long)block * 256 + tid) * 4;
+  if (i >= u.n) return;
+  f32x4 s = *(const f32x4*)(u.parts + i);
+#pragma unroll 4
+  for (int k = 1; k < u.nsplit; ++k) s += *(const f32x4*)(u.parts + (long long)k * u.n + i);
+  put4<F32>(u.out, i, s[0] * u.scale, s[1] * u.scale, s[2] * u.scale, s[3] * u.scale);
 }
 
 // ================================================================================================
@@ -397,24 +407,18 @@ BwdPlan bwd_plan(const TfScoreAttnArgs* a, bool slopes) {
   const int G = a->H / a->Hk;
   p.nqb = (a->Sq + 127) / 128;
   p.nkb = (a->Sk + 127) / 128;
-  // Too few workgroups for 256 CUs: the loops are split until two a CU are there, each with at least four to eight pairs of tiles.  dk / dv are split
-  // by heads first (each is a loop of its own), and up to four a CU: with shared heads a workgroup's loop is long and uneven.
+  // Too few workgroups for 256 CUs: the loops are split.  dk / dv are split by heads first (each is a loop of its own), and up to four a CU:
+  // with shared heads a workgroup's loop is long and uneven.
   const long long bq = (long long)a->B * a->H * p.nqb, bk = (long long)a->B * a->Hk * p.nkb;
-  auto ways = [](long long blocks, long long target, long long most) { return (int)std::max(1ll, std::min(blocks >= target / 2 ? 1 : (target + blocks - 1) / blocks, most)); };
-  p.sq = bq == 0 ? 1 : ways(bq, 512, (a->Sk + 127) / 128);
+  p.sq = split_ways(a->is_f32, a->D, bq, (a->Sk + 31) / 32, 4);
   p.sg = bk == 0 ? 1 : (int)std::max(1ll, std::min({(1024 + bk - 1) / bk, (long long)G, (long long)G * ((a->Sq + 31) / 32) / 8}));
-  p.sk = bk == 0 ? 1 : ways(bk * p.sg, 512, (a->Sq + 127) / 128);
+  p.sk = split_ways(a->is_f32, a->D, bk * p.sg, (a->Sq + 31) / 32, 4);
   const size_t nq = (size_t)a->B * a->Sq * a->H * a->D, nk = (size_t)a->B * a->Sk * a->Hk * a->D, ns = (size_t)p.sg * p.sk;
   p.o_dk = p.sq > 1 ? p.sq * nq : 0;
   p.o_dv = p.o_dk + (ns > 1 ? ns * nk : 0);
   p.o_rows = p.o_dv + (ns > 1 ? ns * nk : 0);
   p.floats = p.o_rows + (slopes ? (size_t)p.sq * a->B * a->H * a->Sq : 0);
   return p;
-}
-
-template <bool F32> void launch_sum(const TfScoreAttnArgs* a, size_t off, long long n, int nsplit, float scale, void* out, hipStream_t st) {
-  TfTraceScope tr("score_sum_kernel", st);
-  hipLaunchKernelGGL(score_sum_kernel<F32>, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, (const float*)a->work + off, n, nsplit, scale, out);
 }
 
 template <bool F32, int HDP> int launch_bwd(const TfScoreAttnArgs* a, hipStream_t st) {
@@ -426,35 +430,39 @@ template <bool F32, int HDP> int launch_bwd(const TfScoreAttnArgs* a, hipStream_
     allow_lds(kern, lds);
     hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), lds, st, *a, pl);
   };
-  if (pl.nqb > 0) {
-    {
-      TfTraceScope tr(F32 ? "score_dq_kernel<fp32>" : "score_dq_kernel<bf16>", st, 1.5 * fl);
-      const int blocks = a->B * a->H * pl.nqb * pl.sq;
-      doc ? go(score_dq_kernel<F32, HDP, true>, blocks) : go(score_dq_kernel<F32, HDP, false>, blocks);
-    }
-    if (pl.sq > 1) launch_sum<F32>(a, 0, (long long)a->B * a->Sq * a->H * a->D, pl.sq, a->scale, a->dq, st);
+  if (const int blocks = a->B * a->H * pl.nqb * pl.sq; blocks > 0) {
+    TfTraceScope tr(F32 ? "score_dq_kernel<fp32>" : "score_dq_kernel<bf16>", st, 1.5 * fl);
+    doc ? go(score_dq_kernel<F32, HDP, true>, blocks) : go(score_dq_kernel<F32, HDP, false>, blocks);
   }
-  if (a->dslopes != nullptr) {
-    TfTraceScope tr("score_dslope_kernel", st);
-    hipLaunchKernelGGL(score_dslope_kernel, dim3(a->H), dim3(256), 0, st, (const float*)a->work + pl.o_rows, a->dslopes, a->B * pl.sq, a->H, a->Sq);
+  if (const int blocks = a->B * a->Hk * pl.nkb * pl.sg * pl.sk; blocks > 0) {
+    TfTraceScope tr(F32 ? "score_dkv_kernel<fp32>" : "score_dkv_kernel<bf16>", st, 2.0 * fl);
+    auto part = [&](auto which) {
+      constexpr int PART = decltype(which)::value;
+      doc ? go(score_dkv_kernel<F32, HDP, PART, true>, blocks) : go(score_dkv_kernel<F32, HDP, PART, false>, blocks);
+    };
+    if constexpr (HDP <= (F32 ? 128 : 192)) part(std::integral_constant<int, 2>{});
+    else { part(std::integral_constant<int, 0>{}); part(std::integral_constant<int, 1>{}); }
   }
-  if (pl.nkb > 0) {
-    {
-      TfTraceScope tr(F32 ? "score_dkv_kernel<fp32>" : "score_dkv_kernel<bf16>", st, 2.0 * fl);
-      const int blocks = a->B * a->Hk * pl.nkb * pl.sg * pl.sk;
-      auto part = [&](auto which) {
-        constexpr int PART = decltype(which)::value;
-        doc ? go(score_dkv_kernel<F32, HDP, PART, true>, blocks) : go(score_dkv_kernel<F32, HDP, PART, false>, blocks);
-      };
-      if constexpr (HDP <= (F32 ? 128 : 192)) part(std::integral_constant<int, 2>{});
-      else { part(std::integral_constant<int, 0>{}); part(std::integral_constant<int, 1>{}); }
-    }
-    const int ns = pl.sg * pl.sk;
-    const long long n = (long long)a->B * a->Sk * a->Hk * a->D;
-    if (ns > 1) {
-      launch_sum<F32>(a, pl.o_dk, n, ns, a->scale, a->dk, st);
-      launch_sum<F32>(a, pl.o_dv, n, ns, 1.0f, a->dv, st);
-    }
+  const int ns = pl.sg * pl.sk;
+  Finish f{};
+  f.rows = (const float*)a->work + pl.o_rows;
+  f.dslopes = a->dslopes;
+  f.heads = a->dslopes != nullptr ? a->H : 0;
+  f.H = a->H;
+  f.Sq = a->Sq;
+  f.planes = a->B * pl.sq;
+  unsigned blocks = f.heads;
+  auto add = [&](int w, size_t off, long long n, int nsplit, float scale, void* out) {
+    const unsigned need = nsplit > 1 ? (unsigned)((n / 4 + 255) / 256) : 0;
+    f.sum[w] = {(const float*)a->work + off, out, n, nsplit, need, scale};
+    blocks += need;
+  };
+  add(0, 0, (long long)a->B * a->Sq * a->H * a->D, pl.sq, a->scale, a->dq);
+  add(1, pl.o_dk, (long long)a->B * a->Sk * a->Hk * a->D, ns, a->scale, a->dk);
+  add(2, pl.o_dv, (long long)a->B * a->Sk * a->Hk * a->D, ns, 1.0f, a->dv);
+  if (blocks > 0) {
+    TfTraceScope tr("score_finish_kernel", st);
+    hipLaunchKernelGGL(score_finish_kernel<F32>, dim3(blocks), dim3(256), 0, st, f);
   }
   return (int)hipGetLastError();
 }
@@ -480,9 +488,5 @@ extern "C" int tf_launch_score_bwd(const TfScoreAttnArgs* a, hipStream_t st) {
       !score_aligned(a->dq, 0, 0, 0, e) || !score_aligned(a->dk, 0, 0, 0, e) || !score_aligned(a->dv, 0, 0, 0, e)) return -7;
   const size_t need = bwd_plan(a, a->dslopes != nullptr).floats * sizeof(float);
   if (need > 0 && (a->work == nullptr || a->work_bytes < need || ((uintptr_t)a->work & 15) != 0)) return -8;
-  if (a->B == 0) {
-    if (a->dslopes != nullptr) hipLaunchKernelGGL(score_dslope_kernel, dim3(a->H), dim3(256), 0, st, (const float*)nullptr, a->dslopes, 0, a->H, 0);
-    return (int)hipGetLastError();
-  }
   return by_head_dim(a, [&](auto f32, auto hdp) { return launch_bwd<decltype(f32)::value, decltype(hdp)::value>(a, st); });
 }
