@@ -462,25 +462,27 @@ template <bool DOC> struct TileWalk {
   }
 };
 
-// One step of a walk over 64-item tiles in halves of 32 items.
-template <bool DOC> struct HalfWalk {
+// A walk over the halves (32 items) [s_lo, items / 32) of 64-item tiles in steps of T = 64 or 32 items.  s: the step in hand starts at item 32 s
+// (a step of 64 at an even half, whether or not the range holds both of its halves: see `mine`), -1 at the end.
+template <bool DOC, int T> struct StepWalk {
   TileWalk<DOC> w;
-  int s, items;                           // s: the half in hand (items 32 s ..), -1 at the end
+  int s, s_lo, items;
   bool full, neg;
-  __device__ __forceinline__ void first(int s0, u64 (*sh)[3], int wave, int lane) {
-    const int t = w.first(s0 >> 1, sh, wave, lane);
-    s = t < 0 ? -1 : max(2 * t, s0);
+  __device__ __forceinline__ void first(u64 (*sh)[3], int wave, int lane) {
+    const int t = w.first(s_lo >> 1, sh, wave, lane);
+    s = t < 0 ? -1 : T == 64 ? 2 * t : max(2 * t, s_lo);
     if (s >= 0 && s * 32 >= items) s = -1;
     full = w.full;
     neg = w.neg;
   }
   __device__ __forceinline__ void next(u64 (*sh)[3], int wave, int lane) {
-    if (!(s & 1) && (s + 1) * 32 < items) { ++s; return; }
+    if (T == 32 && !(s & 1) && (s + 1) * 32 < items) { ++s; return; }
     const int t = w.next(s >> 1, sh, wave, lane);
     s = t < 0 ? -1 : 2 * t;
     full = w.full;
     neg = w.neg;
   }
+  __device__ __forceinline__ bool mine(int half) const { return half >= s_lo && half * 32 < items; }
 };
 
 // range of the documents of a workgroup's 128 rows (d: this lane's row, live: it takes part) for a walk

@@ -7,13 +7,20 @@
 
 namespace {
 
-// Two 32-row tiles that are used together (K and V, or Q and dO) as one image: waves 0 and 1 fetch the first, 2 and 3 the second.  Two
-// images, one barrier a pair: the next pair is under way while one is worked on.  (A third image, transfers waited for by count, gained
-// nothing: 4 x 4096 causal, 8 heads of 128, 653 against 603 us, and 4 x 2048, 16 heads of 64, 308 either way.)
-template <bool F32, int HDP> struct Pair {
-  using Dma = SDma<F32, HDP, 32, 2>;
-  static constexpr int HALF = Dma::BYTES, BUF = 2 * HALF, IMAGES = 2 * BUF;
+// Two tiles of T rows that are used together (K and V, or Q and dO) as one image: waves 0 and 1 fetch the first, 2 and 3 the second.  Two
+// images, one barrier a pair: the next pair is under way while one is worked on, 32 rows at a time.  WG workgroups share a CU's LDS; T is 64
+// where that leaves the room, which halves the barriers (32 x 708, 4 heads of 192: 301 -> 276 us; elsewhere 1 to 2 %).
+// (A third image, transfers waited for by count, gained nothing: 4 x 4096 causal, 8 heads of 128, 653 against 603 us, and 4 x 2048, 16 heads of
+// 64, 308 either way.)
+template <bool F32, int HDP, int WG> struct Pair {
+  static constexpr int EXTRA = 2048;      // statistics and documents of the rows, scan of the documents
+  static constexpr int T = 4 * SDma<F32, HDP, 64, 2>::BYTES + EXTRA <= 160 * 1024 / WG ? 64 : 32;
+  using Dma = SDma<F32, HDP, T, 2>;
+  static constexpr int HALF = Dma::BYTES, BUF = 2 * HALF, IMAGES = 2 * BUF, LDS = IMAGES + EXTRA;
 };
+// workgroups a CU (what the registers allow)
+constexpr int dq_wgs(bool f32, int hdp) { return hdp <= (f32 ? 64 : 128) ? 2 : 1; }
+constexpr int dkv_wgs(bool f32, int hdp, int part) { return hdp <= (f32 ? 32 : part == 2 ? 64 : part == 1 ? 128 : 192) ? 2 : 1; }
 
 // a pair under way: half-tile number (-1: none), full (see TileWalk)
 struct Coming { int s = -1; bool full = false; };
@@ -38,14 +45,14 @@ struct BwdPlan {
 // dq: query on the lane, 128 queries a workgroup; also delta, and the slopes' row sums
 // ================================================================================================
 template <bool F32, int HDP, bool DOC>
-__global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_dq_kernel(const TfScoreAttnArgs a, const BwdPlan pl) {
+__global__ __launch_bounds__(256, dq_wgs(F32, HDP)) void score_dq_kernel(const TfScoreAttnArgs a, const BwdPlan pl) {
   using G = SGeo<F32, HDP>;
-  using PR = Pair<F32, HDP>;
+  using PR = Pair<F32, HDP, dq_wgs(F32, HDP)>;
   // fp32 heads of 256 (of 192 with documents): Q, dO and dq do not fit the register file together; Q and dO are read again (from the caches) for every tile
   constexpr bool REREAD = F32 && (HDP > 192 || (HDP > 128 && DOC));
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 512);
-  int* rsh = (int*)(smem + PR::IMAGES + 512 + 96);
+  u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 1536);
+  int* rsh = (int*)(smem + PR::IMAGES + 1536 + 96);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   int block, group;
   order_blocks(pl.nqb, a.H / a.Hk * pl.sq, a.causal, block, group);
@@ -64,14 +71,14 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_
   const QRow qr = q_row(a, p0, pfx, w0, i);
   const int hi = key_end(a, p0, pfx, min(qb * 128 + 127, a.Sq - 1));
   const int units = (hi + 31) / 32, u_lo = (int)((long long)units * split / pl.sq), u_hi = (int)((long long)units * (split + 1) / pl.sq);
-  HalfWalk<DOC> walk{{kdoc, (u_hi + 1) / 2, a.Sk, 0, 0, 0, {}, true, false}, -1, min(hi, u_hi * 32), true, false};
+  StepWalk<DOC, PR::T> walk{{kdoc, (u_hi + 1) / 2, a.Sk, 0, 0, 0, {}, true, false}, -1, u_lo, min(hi, u_hi * 32), true, false};
   if (DOC) doc_range(qd, live, rsh, wave, lane, walk.w.dmin, walk.w.dmax);
-  walk.first(u_lo, dsh, wave, lane);
+  walk.first(dsh, wave, lane);
   const typename PR::Dma dma(wave & 1, lane, xrb, a.D);
-  int* kds = (int*)(smem + PR::IMAGES);    // [2 images][64] documents of the keys (32 used)
+  int* kds = (int*)(smem + PR::IMAGES);    // [2 images][64] documents of the keys
   auto fetch = [&](int buf) {
     // (keys behind the last are hidden by the row's limit, whatever document they show)
-    if (DOC && wave == 0) __builtin_amdgcn_global_load_lds(TF_GLB_PTR(kdoc + min(walk.s * 32 + (lane & 31), a.Sk - 1)), TF_LDS_PTR(kds + buf * 64), 4, 0, 0);
+    if (DOC && wave == 0) __builtin_amdgcn_global_load_lds(TF_GLB_PTR(kdoc + min(walk.s * 32 + lane, a.Sk - 1)), TF_LDS_PTR(kds + buf * 64), 4, 0, 0);
     dma.issue(xbase, xrb, walk.s * 32, hi, a.D, DOC && walk.neg ? kdoc : nullptr, smem + buf * PR::BUF + (wave >> 1) * PR::HALF);
   };
   const long long row = (long long)bh * a.Sq + ic, orow = (((long long)b * a.Sq + ic) * a.H + head) * a.D;
@@ -123,48 +130,61 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_
   const SAddr<F32, HDP> fk0(lds_addr_of(smem), lane);
   int buf = 0;
   while (cur.s >= 0) {
-    const int kv0 = cur.s * 32;
-    const bool full_t = cur.full && kv0 + 31 <= qr.lim_lo, work = wave_live && kv0 <= qr.lim_hi;
+    unsigned todo = 0;                   // (uniform) halves this wave has work in; 4: all of it is visible
+#pragma unroll
+    for (int hf = 0; hf < PR::T / 32; ++hf) {
+      const int kv0 = (cur.s + hf) * 32;
+      if (wave_live && kv0 <= qr.lim_hi && (PR::T == 32 || walk.mine(cur.s + hf))) todo |= (cur.full && kv0 + 31 <= qr.lim_lo ? 5u : 1u) << hf;
+    }
     dma_wait_barrier();                  // the pair in hand is there, and every wave is done with the one before
     const Coming nxt = go_on(buf ^ 1);
-    if (work) {
-      const SAddr<F32, HDP> fk = fk0.shifted(buf * PR::BUF);
-      f32x16 st, dp;
+    auto rows32 = [&](int hf) __attribute__((always_inline)) {
+      const int kv0 = (cur.s + hf) * 32;
+      if ((todo >> hf) & 1u) {
+        const bool full_t = (todo >> hf) & 4u;
+        const SAddr<F32, HDP> fk = fk0.shifted(buf * PR::BUF + hf * 32 * G::STR);
+        f32x16 st, dp;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = 0.f; }
-      mul_rows2<F32, HDP, PR::HALF>(fk, qx, dx, st, dp);
-      unsigned bits = 0xffffffffu;
-      if (!full_t) {
-        bits = low_bits(qr.lim - kv0 + 1);
-        if (DOC) {
-          unsigned kd = rd32_asm<0>(lds_addr_of(kds + buf * 64) + (lane & 31) * 4);
-          lgkm_wait32<0>(kd);
-          bits &= (unsigned)doc_bits(qd, (int)kd);
+        for (int r = 0; r < 16; ++r) { st[r] = 0.f; dp[r] = 0.f; }
+        mul_rows2<F32, HDP, PR::HALF>(fk, qx, dx, st, dp);
+        unsigned bits = 0xffffffffu;
+        if (!full_t) {
+          bits = low_bits(qr.lim - kv0 + 1);
+          if (DOC) {
+            unsigned kd = rd32_asm<0>(lds_addr_of(kds + buf * 64 + hf * 32) + (lane & 31) * 4);
+            lgkm_wait32<0>(kd);
+            bits &= (unsigned)doc_bits(qd, (int)kd);
+          }
+          bits >>= 4 * h;
         }
-        bits >>= 4 * h;
+        const float pd = (float)(qr.p - kv0 - 4 * h), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
+        SPack<F32> pk[1];
+        const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
+        const int cap = m.capl == 0.f ? 0 : all_small<F32, 1>(m, raw) ? 2 : 1;
+        by_flags(full_t, cap, m.slope2 != 0.f || a.dslopes != nullptr, [&](auto FULL, auto CAP, auto SLP) {
+          auto one = [&](int r) {
+            const int j = (r & 3) + 8 * (r >> 2);
+            float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? capped_exact<F32>(m, st[r]) : st[r] * m.sc, x = t;
+            const float dist = SLP ? fabsf(pd - (float)j) : 0.f;
+            if (SLP) x -= m.slope2 * dist;
+            x = fast_exp2(x - lse) * (dp[r] - delta);
+            if (!FULL) x = (bits >> j) & 1u ? x : 0.f;
+            if (SLP) dsl -= x * dist;
+            return CAP ? x * fmaf(t * t, ncap, 1.0f) : x;           // the cap's derivative: 1 - (t / cap)^2
+          };
+#pragma unroll
+          for (int r = 0; r < 16; r += 2) {
+            const float x0 = one(r), x1 = one(r + 1);
+            pk[0].set2(r, x0, x1);
+          }
+        });
+        fk.template mul_t<0>(pk, dq);
       }
-      const float pd = (float)(qr.p - kv0 - 4 * h), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
-      SPack<F32> pk[1];
-      const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
-      const int cap = m.capl == 0.f ? 0 : all_small<F32, 1>(m, raw) ? 2 : 1;
-      by_flags(full_t, cap, m.slope2 != 0.f || a.dslopes != nullptr, [&](auto FULL, auto CAP, auto SLP) {
-        auto one = [&](int r) {
-          const int j = (r & 3) + 8 * (r >> 2);
-          float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? capped_exact<F32>(m, st[r]) : st[r] * m.sc, x = t;
-          const float dist = SLP ? fabsf(pd - (float)j) : 0.f;
-          if (SLP) x -= m.slope2 * dist;
-          x = fast_exp2(x - lse) * (dp[r] - delta);
-          if (!FULL) x = (bits >> j) & 1u ? x : 0.f;
-          if (SLP) dsl -= x * dist;
-          return CAP ? x * fmaf(t * t, ncap, 1.0f) : x;           // the cap's derivative: 1 - (t / cap)^2
-        };
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) {
-          const float x0 = one(r), x1 = one(r + 1);
-          pk[0].set2(r, x0, x1);
-        }
-      });
-      fk.template mul_t<0>(pk, dq);
+    };
+    if constexpr (PR::T == 32) rows32(0);
+    else {
+#pragma unroll 1
+      for (int hf = 0; hf < 2; ++hf) rows32(hf);
     }
     cur = nxt;
     buf ^= 1;
@@ -186,16 +206,16 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 64 : 128) ? 2 : 1)) void score_
 // dk, dv: key on the lane, 128 keys a workgroup, over the heads that share them and their queries.  PART 0: dv, 1: dk, 2: both
 // ================================================================================================
 template <bool F32, int HDP, int PART, bool DOC>
-__global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1 ? 128 : 192) ? 2 : 1)) void score_dkv_kernel(const TfScoreAttnArgs a, const BwdPlan pl) {
+__global__ __launch_bounds__(256, dkv_wgs(F32, HDP, PART)) void score_dkv_kernel(const TfScoreAttnArgs a, const BwdPlan pl) {
   using G = SGeo<F32, HDP>;
-  using PR = Pair<F32, HDP>;
+  using PR = Pair<F32, HDP, dkv_wgs(F32, HDP, PART)>;
   constexpr bool DK = PART != 0, DV = PART != 1;
   constexpr bool REREAD = F32 && HDP > 192;              // as in score_dq_kernel: V is read again for every tile
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  float* stat = (float*)(smem + PR::IMAGES);             // [2 images][32 lse, 32 delta]
-  int* qds = (int*)(smem + PR::IMAGES + 512);             // [2 images][64] documents of the queries (32 used)
-  u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 1024);
-  int* rsh = (int*)(smem + PR::IMAGES + 1024 + 96);
+  float* stat = (float*)(smem + PR::IMAGES);             // [2 images][64 lse, 64 delta]
+  int* qds = (int*)(smem + PR::IMAGES + 1024);            // [2 images][64] documents of the queries
+  u64 (*dsh)[3] = (u64 (*)[3])(smem + PR::IMAGES + 1536);
+  int* rsh = (int*)(smem + PR::IMAGES + 1536 + 96);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int nsplit = pl.sg * pl.sk;
   int kb, group;
@@ -240,7 +260,7 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1
   const int s_g = split / pl.sk, s_k = split % pl.sk, g_lo = G_ * s_g / pl.sg, g_hi = G_ * (s_g + 1) / pl.sg;
   const int u0 = i_lo / 32, units = (a.Sq + 31) / 32 - u0;
   const int u_lo = u0 + (int)((long long)units * s_k / pl.sk), u_hi = u0 + (int)((long long)units * (s_k + 1) / pl.sk);
-  HalfWalk<DOC> walk{{qdoc, (u_hi + 1) / 2, a.Sq, 0, 0, 0, {}, true, false}, -1, min(a.Sq, u_hi * 32), true, false};
+  StepWalk<DOC, PR::T> walk{{qdoc, (u_hi + 1) / 2, a.Sq, 0, 0, 0, {}, true, false}, -1, u_lo, min(a.Sq, u_hi * 32), true, false};
   if (DOC) doc_range(kd, live, rsh, wave, lane, walk.w.dmin, walk.w.dmax);
   const unsigned xrb = (unsigned)(wave < 2 ? a.q_ss : a.do_ss) * G::ESZ;
   const typename PR::Dma dma(wave & 1, lane, xrb, a.D);
@@ -252,13 +272,13 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1
     const char* xbase = wave < 2 ? (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * G::ESZ
                                  : (const char*)a.dout + ((long long)b * a.do_sb + (long long)head * a.do_sh) * G::ESZ;
     const long long row0 = ((long long)b * a.H + head) * a.Sq;
-    auto fetch = [&](int buf) {           // the pair in walk.s, its rows' statistics (wave 0: 32 of each, 4 bytes a lane) and documents
+    auto fetch = [&](int buf) {           // the pair in walk.s, its rows' statistics (waves 0 and 1) and documents, 4 bytes a lane
       const int i0 = walk.s * 32;
       // (queries behind the last are hidden by number, whatever document they show)
-      if (DOC && wave == 1) __builtin_amdgcn_global_load_lds(TF_GLB_PTR(qdoc + min(i0 + (lane & 31), a.Sq - 1)), TF_LDS_PTR(qds + buf * 64), 4, 0, 0);
-      if (wave == 0) {
-        const float* src = (lane < 32 ? a.lse : a.delta) + row0 + min(i0 + (lane & 31), a.Sq - 1);
-        __builtin_amdgcn_global_load_lds(TF_GLB_PTR(src), TF_LDS_PTR(stat + buf * 64), 4, 0, 0);
+      if (DOC && wave == 2) __builtin_amdgcn_global_load_lds(TF_GLB_PTR(qdoc + min(i0 + lane, a.Sq - 1)), TF_LDS_PTR(qds + buf * 64), 4, 0, 0);
+      if (wave < 2) {
+        const float* src = (wave == 0 ? a.lse : a.delta) + row0 + min(i0 + lane, a.Sq - 1);
+        __builtin_amdgcn_global_load_lds(TF_GLB_PTR(src), TF_LDS_PTR(stat + buf * 128 + wave * 64), 4, 0, 0);
       }
       dma.issue(xbase, xrb, i0, a.Sq, a.D, DOC && walk.neg ? qdoc : nullptr, smem + buf * PR::BUF + (wave >> 1) * PR::HALF);
     };
@@ -273,72 +293,85 @@ __global__ __launch_bounds__(256, (HDP <= (F32 ? 32 : PART == 2 ? 64 : PART == 1
       walk.next(dsh, wave, lane);
       return take(image);
     };
-    walk.first(u_lo, dsh, wave, lane);
+    walk.first(dsh, wave, lane);
     if (g > g_lo) __syncthreads();        // every wave is done with the images of the head before
     int buf = 0;
     cur = take(0);
     while (cur.s >= 0) {
-      const int i0 = cur.s * 32;
-      const bool full_t = cur.full && i0 >= q_full && i0 + 32 <= a.Sq, work = wave_live && i0 + 31 >= q_any;
-      dma_wait_barrier();                  // the pair in hand is there, and every wave is done with the one before
+      unsigned todo = 0;                 // as in score_dq_kernel
+#pragma unroll
+      for (int hf = 0; hf < PR::T / 32; ++hf) {
+        const int i0 = (cur.s + hf) * 32;
+        if (wave_live && i0 + 31 >= q_any && (PR::T == 32 || walk.mine(cur.s + hf))) todo |= (cur.full && i0 >= q_full && i0 + 32 <= a.Sq ? 5u : 1u) << hf;
+      }
+      dma_wait_barrier();                // the pair in hand is there, and every wave is done with the one before
       const Coming nxt = go_on(buf ^ 1);
-      if (work) {
-        const SAddr<F32, HDP> fq = fq0.shifted(buf * PR::BUF);
-        f32x16 st, dp;
+      auto rows32 = [&](int hf) __attribute__((always_inline)) {
+        const int i0 = (cur.s + hf) * 32;
+        if ((todo >> hf) & 1u) {
+          const bool full_t = (todo >> hf) & 4u;
+          const SAddr<F32, HDP> fq = fq0.shifted(buf * PR::BUF + hf * 32 * G::STR);
+          f32x16 st, dp;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) st[r] = 0.f;
-        u32x4 ls[4];                      // register 4 g + e is query 8 g + 4 h + e
-        const unsigned sa = stat0 + buf * 256;
-        static_for<4>([&](auto I) { ls[I] = rd128_asm<32 * I>(sa); });
-        if constexpr (DK) {               // dP - delta: the product starts at -delta
-          u32x4 de[4];
-          static_for<4>([&](auto I) { de[I] = rd128_asm<128 + 32 * I>(sa); });
-          static_for<4>([&](auto I) {
-            lgkm_wait<0>(de[I]);
+          for (int r = 0; r < 16; ++r) st[r] = 0.f;
+          u32x4 ls[4];                      // register 4 g + e is query 8 g + 4 h + e
+          const unsigned sa = stat0 + buf * 512 + hf * 128;
+          static_for<4>([&](auto I) { ls[I] = rd128_asm<32 * I>(sa); });
+          if constexpr (DK) {               // dP - delta: the product starts at -delta
+            u32x4 de[4];
+            static_for<4>([&](auto I) { de[I] = rd128_asm<256 + 32 * I>(sa); });
+            static_for<4>([&](auto I) {
+              lgkm_wait<0>(de[I]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) dp[4 * I + e] = -f_of(de[I][e]);
-          });
-          mul_rows2<F32, HDP, PR::HALF>(fq, kx, vx, st, dp);
-        } else mul_rows<F32, HDP>(fq, kx, st);
-        unsigned bits = 0xffffffffu;
-        if (!full_t) {
-          bits = ~low_bits(max(q_lane - i0, 0)) & low_bits(a.Sq - i0);
-          if (DOC) {
-            unsigned qd = rd32_asm<0>(lds_addr_of(qds + buf * 64) + (lane & 31) * 4);
-            lgkm_wait32<0>(qd);
-            bits &= (unsigned)doc_bits(kd, (int)qd);
-          }
-          bits >>= 4 * h;
-        }
-        static_for<4>([&](auto I) { lgkm_wait<0>(ls[I]); });
-        const float pd = (float)(p0 + i0 + 4 * h - j), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
-        SPack<F32> pp[1], ps[1];
-        const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
-        const int cap = m.capl == 0.f ? 0 : all_small<F32, 1>(m, raw) ? 2 : 1;
-        by_flags(full_t, cap, m.slope2 != 0.f, [&](auto FULL, auto CAP, auto SLP) {
-          auto one = [&](int r, float& pr, float& ds) {
-            const int q = (r & 3) + 8 * (r >> 2);
-            float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? capped_exact<F32>(m, st[r]) : st[r] * m.sc, x = t;
-            if (SLP) x -= m.slope2 * fabsf(pd + (float)q);
-            pr = fast_exp2(x - f_of(ls[r >> 2][r & 3]));
-            if (!FULL) pr = (bits >> q) & 1u ? pr : 0.f;
-            if constexpr (DK) {
-              ds = pr * dp[r];
-              if (CAP) ds *= fmaf(t * t, ncap, 1.0f);
-              if (!FULL) ds = (bits >> q) & 1u ? ds : 0.f;        // (a hidden pair's product may not be finite)
+              for (int e = 0; e < 4; ++e) dp[4 * I + e] = -f_of(de[I][e]);
+            });
+            mul_rows2<F32, HDP, PR::HALF>(fq, kx, vx, st, dp);
+          } else mul_rows<F32, HDP>(fq, kx, st);
+          unsigned bits = 0xffffffffu;
+          if (!full_t) {
+            bits = ~low_bits(max(q_lane - i0, 0)) & low_bits(a.Sq - i0);
+            if (DOC) {
+              unsigned qd = rd32_asm<0>(lds_addr_of(qds + buf * 64 + hf * 32) + (lane & 31) * 4);
+              lgkm_wait32<0>(qd);
+              bits &= (unsigned)doc_bits(kd, (int)qd);
             }
-          };
-#pragma unroll
-          for (int r = 0; r < 16; r += 2) {
-            float p0_, p1_, s0_ = 0.f, s1_ = 0.f;
-            one(r, p0_, s0_);
-            one(r + 1, p1_, s1_);
-            if constexpr (DV) pp[0].set2(r, p0_, p1_);
-            if constexpr (DK) ps[0].set2(r, s0_, s1_);
+            bits >>= 4 * h;
           }
-        });
-        if constexpr (DV) fq.template mul_t<PR::HALF>(pp, dv);
-        if constexpr (DK) fq.template mul_t<0>(ps, dk);
+          static_for<4>([&](auto I) { lgkm_wait<0>(ls[I]); });
+          const float pd = (float)(p0 + i0 + 4 * h - j), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
+          SPack<F32> pp[1], ps[1];
+          const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
+          const int cap = m.capl == 0.f ? 0 : all_small<F32, 1>(m, raw) ? 2 : 1;
+          by_flags(full_t, cap, m.slope2 != 0.f, [&](auto FULL, auto CAP, auto SLP) {
+            auto one = [&](int r, float& pr, float& ds) {
+              const int q = (r & 3) + 8 * (r >> 2);
+              float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? capped_exact<F32>(m, st[r]) : st[r] * m.sc, x = t;
+              if (SLP) x -= m.slope2 * fabsf(pd + (float)q);
+              pr = fast_exp2(x - f_of(ls[r >> 2][r & 3]));
+              if (!FULL) pr = (bits >> q) & 1u ? pr : 0.f;
+              if constexpr (DK) {
+                ds = pr * dp[r];
+                if (CAP) ds *= fmaf(t * t, ncap, 1.0f);
+                if (!FULL) ds = (bits >> q) & 1u ? ds : 0.f;        // (a hidden pair's product may not be finite)
+              }
+            };
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+              float p0_, p1_, s0_ = 0.f, s1_ = 0.f;
+              one(r, p0_, s0_);
+              one(r + 1, p1_, s1_);
+              if constexpr (DV) pp[0].set2(r, p0_, p1_);
+              if constexpr (DK) ps[0].set2(r, s0_, s1_);
+            }
+          });
+          if constexpr (DV) fq.template mul_t<PR::HALF>(pp, dv);
+          if constexpr (DK) fq.template mul_t<0>(ps, dk);
+        }
+      };
+      if constexpr (PR::T == 32) rows32(0);
+      else {
+#pragma unroll 1
+        for (int hf = 0; hf < 2; ++hf) rows32(hf);
       }
       cur = nxt;
       buf ^= 1;
@@ -425,20 +458,21 @@ template <bool F32, int HDP> int launch_bwd(const TfScoreAttnArgs* a, hipStream_
   const double fl = 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D;
   const BwdPlan pl = bwd_plan(a, a->dslopes != nullptr);
   const bool doc = a->k_doc != nullptr;
-  const size_t lds = Pair<F32, HDP>::IMAGES + 1024 + 128;
-  auto go = [&](auto kern, int blocks) {
+  auto go = [&](auto kern, int blocks, size_t lds) {
     allow_lds(kern, lds);
     hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), lds, st, *a, pl);
   };
   if (const int blocks = a->B * a->H * pl.nqb * pl.sq; blocks > 0) {
     TfTraceScope tr(F32 ? "score_dq_kernel<fp32>" : "score_dq_kernel<bf16>", st, 1.5 * fl);
-    doc ? go(score_dq_kernel<F32, HDP, true>, blocks) : go(score_dq_kernel<F32, HDP, false>, blocks);
+    constexpr size_t lds = Pair<F32, HDP, dq_wgs(F32, HDP)>::LDS;
+    doc ? go(score_dq_kernel<F32, HDP, true>, blocks, lds) : go(score_dq_kernel<F32, HDP, false>, blocks, lds);
   }
   if (const int blocks = a->B * a->Hk * pl.nkb * pl.sg * pl.sk; blocks > 0) {
     TfTraceScope tr(F32 ? "score_dkv_kernel<fp32>" : "score_dkv_kernel<bf16>", st, 2.0 * fl);
     auto part = [&](auto which) {
       constexpr int PART = decltype(which)::value;
-      doc ? go(score_dkv_kernel<F32, HDP, PART, true>, blocks) : go(score_dkv_kernel<F32, HDP, PART, false>, blocks);
+      constexpr size_t lds = Pair<F32, HDP, dkv_wgs(F32, HDP, PART)>::LDS;
+      doc ? go(score_dkv_kernel<F32, HDP, PART, true>, blocks, lds) : go(score_dkv_kernel<F32, HDP, PART, false>, blocks, lds);
     };
     if constexpr (HDP <= (F32 ? 128 : 192)) part(std::integral_constant<int, 2>{});
     else { part(std::integral_constant<int, 0>{}); part(std::integral_constant<int, 1>{}); }
