@@ -173,8 +173,11 @@ template <bool F32, int HDP, int ROWS, int NW> struct SDma {
 #pragma unroll
       for (int i = 0; i < NI; ++i) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TF_LDS_PTR(dst + i * 1024), 16, (int)off[i], 0, 0, 0);
     } else {
+      // (a lane a row and one ballot: a load a piece, each waited for, took as long as the tile's products)
+      const u64 neg = doc != nullptr ? __ballot(doc[row0 + min(lane, n - 1)] < 0) : 0ull;
+#pragma unroll 1
       for (int i = 0; i < NI; ++i) {
-        const unsigned o = doc != nullptr && doc[row0 + min(slot(i) / T, n - 1)] < 0 ? OUT : offset(i, row_bytes, D);
+        const unsigned o = (neg >> min(slot(i) / T, 63)) & 1ull ? OUT : offset(i, row_bytes, D);
         __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, TF_LDS_PTR(dst + i * 1024), 16, (int)o, 0, 0, 0);
       }
     }
