@@ -145,6 +145,14 @@ CASES = {
     "token caches": (4, 1, 1000, 8, 2, 96, {"causal": 1, "start": 1, "prefix": 1}),
     "32 rows": (2, 4, 222, 8, 1, 128, {"causal": 1}),
     "33 rows": (2, 33, 222, 1, 1, 32, {"causal": 1}),
+    "cap tiny": (1, 70, 70, 2, 1, 64, {"cap": 1e-10, "causal": 1}),
+    "cap huge": (1, 70, 70, 2, 1, 64, {"cap": 1e10, "causal": 1}),
+    "sets of eight": (8, 150, 150, 2, 1, 32, {"causal": 1}),             # every way in which causal blocks are dealt
+    "eight heads": (2, 150, 150, 4, 2, 32, {"causal": 1, "pad": 1}),
+    "eight parts": (1, 700, 700, 2, 2, 24, {"causal": 1}),
+    "odd halves": (1, 353, 290, 2, 1, 64, {"causal": 1, "slopes": 1}),   # parts of a loop that begin inside a tile
+    "odd halves documents": (1, 419, 419, 2, 2, 192, {"causal": 1, "docs": 3, "pad": 1}),
+    "odd halves wide": (1, 290, 353, 3, 3, 128, {"docs": 2, "pad": 1}),
     "few rows split": (1, 40, 2100, 2, 1, 64, {"causal": 1, "slopes": 1, "pad": 1}),
 }
 
@@ -539,7 +547,7 @@ def test_refusals(dev):
     i = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)
     for args, kw in [((q, k, k[:, :6]), {}), ((q, k[:1], k[:1]), {}), ((q[0], k, k), {}), ((q, k.to(BF), k.to(BF)), {}), ((q.half(), k.half(), k.half()), {}),
                      ((q[:, :, :3], k, k), {}), ((q[..., :12], k[..., :12], k[..., :12]), {}), ((q, k.cpu(), k), {}), ((q, k, k), {"softcap": -1.0}),
-                     ((q, k, k), {"softcap": math.inf}), ((q, k, k), {"scale": math.nan}), ((q, k, k), {"slopes": torch.zeros(2, device=dev)}),
+                     ((q, k, k), {"softcap": math.inf}), ((q, k, k), {"softcap": 1e-11}), ((q, k, k), {"softcap": 1e11}), ((q, k, k), {"scale": 1e11}), ((q, k, k), {"scale": math.nan}), ((q, k, k), {"slopes": torch.zeros(2, device=dev)}),
                      ((q, k, k), {"slopes": torch.zeros(4)}), ((q, k, k), {"slopes": torch.zeros(4, dtype=BF, device=dev)}), ((q, k, k), {"prefix": i(2)}),
                      ((q, k, k), {"causal": True, "prefix": i(3)}), ((q, k, k), {"causal": True, "prefix": torch.zeros(2, dtype=torch.int64, device=dev)}),
                      ((q, k, k), {"causal": True, "q_start": 3}), ((q, k, k), {"q_doc": i(2, 5)}), ((q, k, k), {"q_doc": i(2, 5), "k_doc": i(2, 5)})]:

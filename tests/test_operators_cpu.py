@@ -43,6 +43,7 @@ def attn_args(**kw):
 
 
 BOTH = [dict(H=0), dict(Hk=0), dict(Hk=3), dict(D=0), dict(D=12), dict(D=264), dict(B=-1), dict(Sq=-1), dict(Sk=-1), dict(softcap=-1.0),
+        dict(softcap=math.inf), dict(softcap=1e-11), dict(softcap=1e11), dict(scale=math.inf), dict(scale=math.nan), dict(scale=-1e11),
         dict(softcap=math.nan), dict(q_doc=PTR), dict(k_doc=PTR), dict(q=0), dict(k=0), dict(v=0), dict(out=0), dict(q=PTR + 8), dict(k_ss=60), dict(v_sh=4),
         dict(q_sb=4), dict(B=1 << 20, Sq=1 << 10), dict(Sk=1 << 30)]
 

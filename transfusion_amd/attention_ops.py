@@ -260,8 +260,8 @@ def score_attention(q, k, v, scale: float = None, softcap: float = 0.0, slopes=N
         raise L.TfError(f"score_attention: head_dim {D} must be a multiple of 8, at most 256")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     softcap = float(softcap)
-    if not math.isfinite(scale) or not (0.0 <= softcap < math.inf):
-        raise L.TfError(f"score_attention: scale {scale} must be finite, softcap {softcap} finite and not negative")
+    if not abs(scale) <= 1e10 or not (softcap == 0.0 or 1e-10 <= softcap <= 1e10):
+        raise L.TfError(f"score_attention: scale {scale} must lie within 1e10 of 0, softcap {softcap} be 0 (none) or between 1e-10 and 1e10")
     dev = q.device
     if slopes is not None:
         ops._require_cuda(slopes)

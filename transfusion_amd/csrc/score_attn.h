@@ -562,7 +562,8 @@ inline int split_ways(bool f32, int D, long long blocks, long long units, int le
 inline int score_check(const TfScoreAttnArgs* a) {
   if (a->B < 0 || a->Sq < 0 || a->Sk < 0 || a->H <= 0 || a->Hk <= 0 || a->H % a->Hk != 0) return -1;
   if (a->D <= 0 || a->D > 256 || a->D % 8 != 0) return -2;
-  if (!(a->softcap >= 0.f)) return -3;
+  // (their quotient and its square stay finite)
+  if (!(fabsf(a->scale) <= 1e10f) || !(a->softcap == 0.f || (a->softcap >= 1e-10f && a->softcap <= 1e10f))) return -3;
   if ((a->k_doc == nullptr) != (a->q_doc == nullptr) && a->Sq > 0 && a->Sk > 0) return -4;
   const long long blocks = (long long)a->B * std::max(a->H * ((a->Sq + 127ll) / 128), (long long)a->Hk * ((a->Sk + 127) / 128));
   if (blocks > 0x3fffff || (long long)a->Sq + a->Sk > (1ll << 30)) return -5;
