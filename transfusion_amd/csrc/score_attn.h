@@ -11,8 +11,8 @@
 //   score_attn_bwd.hip   score_dq_kernel: query on the lane -> dq, delta = rowsum(dO o), the slopes' row sums;
 //                        score_dkv_kernel: key on the lane, loops over the heads of its group and their queries -> dk, dv
 // Where there are too few workgroups, a kernel splits its loop and writes fp32 parts that a second kernel adds up in order: no atomics.
-// Scores, statistics and accumulators are fp32.  P and dS are rounded to the operand type of the next product (bf16: half a step, 2^-9
-// of each term); fp32 tensors run on the fp32 matrix instructions throughout.
+// Scores, statistics and accumulators are fp32.  P and dS are rounded to the operand type of the next product (bf16: at most half a step,
+// 2^-8 of each term, as every product of bf16 operands has it already); fp32 tensors run on the fp32 matrix instructions throughout.
 #pragma once
 #include "tf_common.h"
 #include "tf_kernels.h"
@@ -499,6 +499,8 @@ __device__ __forceinline__ void doc_range(int d, bool live, int* sh, int wave, i
 // Which block of rows (0: the one that sees most) and which group this workgroup has; `per` consecutive groups share keys.  Where the blocks differ
 // in work (causal), the heaviest of ALL groups come first, so that the light ones fill up the end.  A chiplet keeps the groups that share
 // keys (workgroups are dealt to the 8 chiplets in turn) and, where they divide evenly, takes samples with stride 8, for the sake of ragged lengths.
+// Against one head after the other (heaviest block first within each): 4 x 4096 causal, 8 heads of 128, forward 170 -> 152 us; 32 x 708 with a
+// prefix, 4 heads of 192, backward 272 -> 226; documents in 8192 tokens, 16 heads of 64, forward 107 -> 92, backward 349 -> 294.
 __device__ __forceinline__ void order_blocks(int nb, int per, bool uneven, int& block, int& group) {
   const int n = gridDim.x / nb;
   if (!uneven) {

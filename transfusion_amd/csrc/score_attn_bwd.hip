@@ -3,6 +3,12 @@
 //   dQ = scale dS K ;  dK = scale dS^T Q .
 // Two kernels, each with every score of its own rows or keys: seven products where five would do, but no gradient is touched by two
 // workgroups, nothing is atomic, and the [Sq, Sk] tensor dS stays out of memory.
+//
+// Bound by the registers: accumulators and row operands leave room for one wave a SIMD from 96 channels (dk / dv) or 192 (dq) on, so the products,
+// the exponentials and the barriers of a tile follow each other more than they overlap (dk / dv at 128 channels: matrix pipe busy 31 % of the
+// time, vector pipe 25 %).  4 x 4096 causal, 8 heads of 128: 575 us = 600 TFLOP/s (five products credited, seven computed); 4 x 2048, 16 heads of
+// 64: 298 us = 575; 32 x 708, 4 heads of 192: 276 us = 445.  Two forms that were no faster: a tile shared by two waves of a SIMD, P handed over
+// through LDS (the first size 606 us where this form took 603), and the next tile's scores formed under this one's products (spilled).
 #include "score_attn.h"
 
 namespace {
@@ -13,7 +19,7 @@ namespace {
 // (A third image, transfers waited for by count, gained nothing: 4 x 4096 causal, 8 heads of 128, 653 against 603 us, and 4 x 2048, 16 heads of
 // 64, 308 either way.)
 template <bool F32, int HDP, int WG> struct Pair {
-  static constexpr int EXTRA = 2048;      // statistics and documents of the rows, scan of the documents
+  static constexpr int EXTRA = 6144;      // statistics and documents of the rows, scan of the documents; from 2048 on the slopes' sums
   static constexpr int T = 4 * SDma<F32, HDP, 64, 2>::BYTES + EXTRA <= 160 * 1024 / WG ? 64 : 32;
   using Dma = SDma<F32, HDP, T, 2>;
   static constexpr int HALF = Dma::BYTES, BUF = 2 * HALF, IMAGES = 2 * BUF, LDS = IMAGES + EXTRA;
@@ -126,7 +132,11 @@ __global__ __launch_bounds__(256, dq_wgs(F32, HDP)) void score_dq_kernel(const T
   for (int d = 0; d < G::DB; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
-  std::conditional_t<F32, double, float> dsl = 0;        // (distances up to the length times small terms of both signs)
+  // The slopes' gradient of a row is -cov(dP, dist) under P.  Its own sums of P, P e, P dist and P e dist (e = dP - delta) make it exact to fp32: delta
+  // holds the roundings of P and of the output, and the mean distance -- hundreds -- would multiply them (2e-3 of the gradient)
+  // (in LDS, a tile's sums at a time: the registers are taken)
+  f32x4* const sums = (f32x4*)(smem + PR::IMAGES + 2048) + tid;
+  if (a.dslopes != nullptr) *sums = f32x4{0, 0, 0, 0};
   const SAddr<F32, HDP> fk0(lds_addr_of(smem), lane);
   int buf = 0;
   while (cur.s >= 0) {
@@ -161,15 +171,24 @@ __global__ __launch_bounds__(256, dq_wgs(F32, HDP)) void score_dq_kernel(const T
         SPack<F32> pk[1];
         const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
         const int cap = m.capl == 0.f ? 0 : all_small<F32, 1>(m, raw) ? 2 : 1;
-        by_flags(full_t, cap, m.slope2 != 0.f || a.dslopes != nullptr, [&](auto FULL, auto CAP, auto SLP) {
+        auto form = [&](auto FULL, auto CAP, auto SLP, auto SUMS) {
+          f32x4 t4 = {0, 0, 0, 0};
           auto one = [&](int r) {
             const int j = (r & 3) + 8 * (r >> 2);
-            float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? capped_exact<F32>(m, st[r]) : st[r] * m.sc, x = t;
+            // (sums: the cap as exactly as fp32 has it)
+            float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? capped_exact<F32 || SUMS>(m, st[r]) : st[r] * m.sc, x = t;
             const float dist = SLP ? fabsf(pd - (float)j) : 0.f;
             if (SLP) x -= m.slope2 * dist;
-            x = fast_exp2(x - lse) * (dp[r] - delta);
+            float pr = fast_exp2(x - lse);
+            x = pr * (dp[r] - delta);
             if (!FULL) x = (bits >> j) & 1u ? x : 0.f;
-            if (SLP) dsl -= x * dist;
+            if (SUMS) {
+              pr = (bits >> j) & 1u ? pr : 0.f;
+              t4[0] += pr;
+              t4[1] += x;
+              t4[2] = fmaf(pr, dist, t4[2]);
+              t4[3] = fmaf(x, dist, t4[3]);
+            }
             return CAP ? x * fmaf(t * t, ncap, 1.0f) : x;           // the cap's derivative: 1 - (t / cap)^2
           };
 #pragma unroll
@@ -177,7 +196,12 @@ __global__ __launch_bounds__(256, dq_wgs(F32, HDP)) void score_dq_kernel(const T
             const float x0 = one(r), x1 = one(r + 1);
             pk[0].set2(r, x0, x1);
           }
-        });
+          if (SUMS) *sums += t4;
+        };
+        if (a.dslopes != nullptr) {           // (one form for full and masked tiles)
+          if (cap != 0) form(std::false_type{}, std::integral_constant<int, 1>{}, std::true_type{}, std::true_type{});
+          else form(std::false_type{}, std::integral_constant<int, 0>{}, std::true_type{}, std::true_type{});
+        } else by_flags(full_t, cap, m.slope2 != 0.f, [&](auto FULL, auto CAP, auto SLP) { form(FULL, CAP, SLP, std::false_type{}); });
         fk.template mul_t<0>(pk, dq);
       }
     };
@@ -189,12 +213,20 @@ __global__ __launch_bounds__(256, dq_wgs(F32, HDP)) void score_dq_kernel(const T
     cur = nxt;
     buf ^= 1;
   }
-  dsl += __shfl_xor(dsl, 32, 64);
   const long long rows = (long long)a.B * a.H * a.Sq;
-  if (i < a.Sq && h == 0) {
-    if (split == 0) a.delta[row] = delta;
-    if (a.dslopes != nullptr) ((float*)a.work)[pl.o_rows + split * rows + row] = live ? (float)dsl : 0.f;
+  if (a.dslopes != nullptr) {
+    f32x4 t = *sums;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] += __shfl_xor(t[e], 32, 64);
+    if (i < a.Sq && h == 0) {
+      float* r = (float*)a.work + pl.o_rows + 4 * split * rows + row;
+      r[0] = live ? t[0] : 0.f;
+      r[rows] = t[1];
+      r[2 * rows] = t[2];
+      r[3 * rows] = t[3];
+    }
   }
+  if (i < a.Sq && h == 0 && split == 0) a.delta[row] = delta;
 #pragma unroll
   for (int d = 0; d < G::DB; ++d)
 #pragma unroll
@@ -395,12 +427,12 @@ __global__ __launch_bounds__(256, dkv_wgs(F32, HDP, PART)) void score_dkv_kernel
 }
 
 // What is left when dq, dk and dv are there, in one launch: the sums of a split gradient's parts (out = scale * (part 0 + part 1 + ...), rounded once; 1024
-// values a workgroup) and, by the first H workgroups, the slopes' gradient: a head's row sums over all samples and parts, in 64 bits and one order.
+// values a workgroup) and, by the first H workgroups, the slopes' gradient: from the four sums of each of its rows, in 64 bits and one order.
 struct Finish {
   struct Sum { const float* parts; void* out; long long n; int nsplit; unsigned blocks; float scale; } sum[3];
   const float* rows;
   float* dslopes;
-  unsigned heads, H, Sq, planes;         // heads: H, or 0 without slopes; planes: samples times parts, [planes][H][Sq]
+  unsigned heads, B, H, Sq, parts;       // heads: H, or 0 without slopes; rows: [parts][P, P e, P dist, P e dist][B][H][Sq]
 };
 template <bool F32> __global__ __launch_bounds__(256) void score_finish_kernel(const Finish f) {
   const int tid = threadIdx.x;
@@ -408,9 +440,20 @@ template <bool F32> __global__ __launch_bounds__(256) void score_finish_kernel(c
   if (block < f.heads) {
     __shared__ double sh[256];
     double s = 0.0;
-    const unsigned n = f.planes * f.Sq;   // (fits: H * n row sums at 128 a workgroup)
-#pragma unroll 8
-    for (unsigned i = tid; i < n; i += 256) s += (double)f.rows[((size_t)(i / f.Sq) * f.H + block) * f.Sq + i % f.Sq];
+    const unsigned n = f.B * f.Sq;        // (fits: H * n rows at 128 a workgroup)
+    const size_t rows = (size_t)n * f.H;
+#pragma unroll 2
+    for (unsigned i = tid; i < n; i += 256) {
+      const float* r = f.rows + ((size_t)(i / f.Sq) * f.H + block) * f.Sq + i % f.Sq;
+      double p = 0.0, e = 0.0, d = 0.0, ed = 0.0;
+      for (unsigned k = 0; k < f.parts; ++k, r += 4 * rows) {
+        p += (double)r[0];
+        e += (double)r[rows];
+        d += (double)r[2 * rows];
+        ed += (double)r[3 * rows];
+      }
+      if (p > 0.0) s -= (ed - e * d / p) / p;             // -cov(e, dist); a row that sees nothing has none
+    }
     sh[tid] = s;
     __syncthreads();
     for (int o = 128; o > 0; o >>= 1) {
@@ -450,7 +493,7 @@ BwdPlan bwd_plan(const TfScoreAttnArgs* a, bool slopes) {
   p.o_dk = p.sq > 1 ? p.sq * nq : 0;
   p.o_dv = p.o_dk + (ns > 1 ? ns * nk : 0);
   p.o_rows = p.o_dv + (ns > 1 ? ns * nk : 0);
-  p.floats = p.o_rows + (slopes ? (size_t)p.sq * a->B * a->H * a->Sq : 0);
+  p.floats = p.o_rows + (slopes ? 4 * (size_t)p.sq * a->B * a->H * a->Sq : 0);
   return p;
 }
 
@@ -484,7 +527,8 @@ template <bool F32, int HDP> int launch_bwd(const TfScoreAttnArgs* a, hipStream_
   f.heads = a->dslopes != nullptr ? a->H : 0;
   f.H = a->H;
   f.Sq = a->Sq;
-  f.planes = a->B * pl.sq;
+  f.B = a->B;
+  f.parts = pl.sq;
   unsigned blocks = f.heads;
   auto add = [&](int w, size_t off, long long n, int nsplit, float scale, void* out) {
     const unsigned need = nsplit > 1 ? (unsigned)((n / 4 + 255) / 256) : 0;
