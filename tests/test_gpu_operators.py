@@ -204,6 +204,17 @@ def test_attention(dev, guard, name, dtype):
         check(n, gr, want[n])
 
 
+@pytest.mark.parametrize("name", [n for n, c in CASES.items() if "slopes" in c[6]])
+def test_attention_slopes_gradient_of_bf16_is_exact_to_fp32(dev, name):
+    """It is an fp32 tensor: no rounding of P, dS or the output to bf16 may reach it, so it has to keep the bounds that the same inputs held in
+    fp32 have."""
+    from transfusion_amd import attention_ops as A
+    q, k, v, go, opt = make(name, BF, lambda t: t.to(dev))
+    want = attention_ref(q.float(), k.float(), v.float(), go.float(), **opt)
+    out = A.score_attention(q, k, v, **{**opt, "slopes": opt["slopes"].requires_grad_(True)})
+    check("dslopes", torch.autograd.grad(out, opt["slopes"], go)[0], want["dslopes"])
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_attention_reads_views(dev, dtype):
     """A packed projection's thirds, heads before tokens, broadcast keys (their gradient is summed by autograd), rows off 16 bytes."""
