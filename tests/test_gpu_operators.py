@@ -153,6 +153,7 @@ CASES = {
     "odd halves": (1, 353, 290, 2, 1, 64, {"causal": 1, "slopes": 1}),   # parts of a loop that begin inside a tile
     "odd halves documents": (1, 419, 419, 2, 2, 192, {"causal": 1, "docs": 3, "pad": 1}),
     "odd halves wide": (1, 290, 353, 3, 3, 128, {"docs": 2, "pad": 1}),
+    "many rows": (3, 500, 500, 2, 1, 16, {"causal": 1, "slopes": 1}),    # more rows than one workgroup adds up
     "few rows split": (1, 40, 2100, 2, 1, 64, {"causal": 1, "slopes": 1, "pad": 1}),
 }
 

@@ -43,8 +43,9 @@ template <bool F32, int DB> __device__ __forceinline__ void store_grad(void* out
 
 // where the parts of the three gradients and of the slopes' row sums lie in the workspace
 struct BwdPlan {
+  unsigned chunks;                       // of the slopes' rows
   int nqb, nkb, sq, sg, sk;              // splits of dq (keys); of dk / dv: groups of heads x ranges of queries
-  size_t o_dk, o_dv, o_rows, floats;
+  size_t o_dk, o_dv, o_rows, o_part, floats;
 };
 
 // ================================================================================================
@@ -432,35 +433,58 @@ struct Finish {
   struct Sum { const float* parts; void* out; long long n; int nsplit; unsigned blocks; float scale; } sum[3];
   const float* rows;
   float* dslopes;
-  unsigned heads, B, H, Sq, parts;       // heads: H, or 0 without slopes; rows: [parts][P, P e, P dist, P e dist][B][H][Sq]
+  double* part;
+  // heads: H, or 0 without slopes; rows: [parts][P, P e, P dist, P e dist][B][H][Sq]; part: [H][chunks] sums of SLOPE_CHUNK rows each where there
+  // are more than one
+  unsigned heads, B, H, Sq, parts, chunks;
 };
+// adds up what 256 threads hold, in one order
+__device__ __forceinline__ double block_sum(double s, int tid) {
+  __shared__ double sh[256];
+  sh[tid] = s;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if (tid < o) sh[tid] += sh[tid + o];
+    __syncthreads();
+  }
+  return sh[0];
+}
+// rows lo .. hi - 1 of the B * Sq of a head
+__device__ __forceinline__ double slope_rows(const Finish& f, unsigned head, unsigned lo, unsigned hi, int tid) {
+  const size_t rows = (size_t)f.B * f.Sq * f.H;
+  double s = 0.0;
+#pragma unroll 2
+  for (unsigned i = lo + tid; i < hi; i += 256) {
+    const float* r = f.rows + ((size_t)(i / f.Sq) * f.H + head) * f.Sq + i % f.Sq;
+    double p = 0.0, e = 0.0, d = 0.0, ed = 0.0;
+#pragma unroll 4
+    for (unsigned k = 0; k < f.parts; ++k, r += 4 * rows) {
+      p += (double)r[0];
+      e += (double)r[rows];
+      d += (double)r[2 * rows];
+      ed += (double)r[3 * rows];
+    }
+    if (p > 0.0) s -= (ed - e * d / p) / p;               // -cov(e, dist); a row that sees nothing has none
+  }
+  return block_sum(s, tid);
+}
+// many rows: a workgroup takes SLOPE_CHUNK rows of a head (one workgroup a head would need half a microsecond for 256 of them)
+constexpr unsigned SLOPE_CHUNK = 1024;
+__global__ __launch_bounds__(256) void score_slope_kernel(const Finish f) {
+  const unsigned head = blockIdx.x / f.chunks, c = blockIdx.x % f.chunks;
+  const double s = slope_rows(f, head, c * SLOPE_CHUNK, min(f.B * f.Sq, (c + 1) * SLOPE_CHUNK), threadIdx.x);
+  if (threadIdx.x == 0) f.part[blockIdx.x] = s;
+}
 template <bool F32> __global__ __launch_bounds__(256) void score_finish_kernel(const Finish f) {
   const int tid = threadIdx.x;
   unsigned block = blockIdx.x;
   if (block < f.heads) {
-    __shared__ double sh[256];
     double s = 0.0;
-    const unsigned n = f.B * f.Sq;        // (fits: H * n rows at 128 a workgroup)
-    const size_t rows = (size_t)n * f.H;
-#pragma unroll 2
-    for (unsigned i = tid; i < n; i += 256) {
-      const float* r = f.rows + ((size_t)(i / f.Sq) * f.H + block) * f.Sq + i % f.Sq;
-      double p = 0.0, e = 0.0, d = 0.0, ed = 0.0;
-      for (unsigned k = 0; k < f.parts; ++k, r += 4 * rows) {
-        p += (double)r[0];
-        e += (double)r[rows];
-        d += (double)r[2 * rows];
-        ed += (double)r[3 * rows];
-      }
-      if (p > 0.0) s -= (ed - e * d / p) / p;             // -cov(e, dist); a row that sees nothing has none
-    }
-    sh[tid] = s;
-    __syncthreads();
-    for (int o = 128; o > 0; o >>= 1) {
-      if (tid < o) sh[tid] += sh[tid + o];
-      __syncthreads();
-    }
-    if (tid == 0) f.dslopes[block] = (float)sh[0];
+    if (f.chunks > 1) {
+      for (unsigned c = tid; c < f.chunks; c += 256) s += f.part[block * f.chunks + c];
+      s = block_sum(s, tid);
+    } else s = slope_rows(f, block, 0, f.B * f.Sq, tid);
+    if (tid == 0) f.dslopes[block] = (float)s;
     return;
   }
   block -= f.heads;
@@ -493,7 +517,9 @@ BwdPlan bwd_plan(const TfScoreAttnArgs* a, bool slopes) {
   p.o_dk = p.sq > 1 ? p.sq * nq : 0;
   p.o_dv = p.o_dk + (ns > 1 ? ns * nk : 0);
   p.o_rows = p.o_dv + (ns > 1 ? ns * nk : 0);
-  p.floats = p.o_rows + (slopes ? 4 * (size_t)p.sq * a->B * a->H * a->Sq : 0);
+  p.chunks = slopes ? (unsigned)(((long long)a->B * a->Sq + SLOPE_CHUNK - 1) / SLOPE_CHUNK) : 0;
+  p.o_part = (p.o_rows + (slopes ? 4 * (size_t)p.sq * a->B * a->H * a->Sq : 0) + 1) / 2 * 2;
+  p.floats = p.o_part + (p.chunks > 1 ? 2 * (size_t)p.chunks * a->H : 0);
   return p;
 }
 
@@ -529,6 +555,8 @@ template <bool F32, int HDP> int launch_bwd(const TfScoreAttnArgs* a, hipStream_
   f.Sq = a->Sq;
   f.B = a->B;
   f.parts = pl.sq;
+  f.chunks = pl.chunks;
+  f.part = (double*)((float*)a->work + pl.o_part);
   unsigned blocks = f.heads;
   auto add = [&](int w, size_t off, long long n, int nsplit, float scale, void* out) {
     const unsigned need = nsplit > 1 ? (unsigned)((n / 4 + 255) / 256) : 0;
@@ -538,6 +566,10 @@ template <bool F32, int HDP> int launch_bwd(const TfScoreAttnArgs* a, hipStream_
   add(0, 0, (long long)a->B * a->Sq * a->H * a->D, pl.sq, a->scale, a->dq);
   add(1, pl.o_dk, (long long)a->B * a->Sk * a->Hk * a->D, ns, a->scale, a->dk);
   add(2, pl.o_dv, (long long)a->B * a->Sk * a->Hk * a->D, ns, 1.0f, a->dv);
+  if (f.heads > 0 && f.chunks > 1) {
+    TfTraceScope tr("score_slope_kernel", st);
+    hipLaunchKernelGGL(score_slope_kernel, dim3(f.heads * f.chunks), dim3(256), 0, st, f);
+  }
   if (blocks > 0) {
     TfTraceScope tr("score_finish_kernel", st);
     hipLaunchKernelGGL(score_finish_kernel<F32>, dim3(blocks), dim3(256), 0, st, f);
