@@ -154,6 +154,7 @@ CASES = {
     "odd halves documents": (1, 419, 419, 2, 2, 192, {"causal": 1, "docs": 3, "pad": 1}),
     "odd halves wide": (1, 290, 353, 3, 3, 128, {"docs": 2, "pad": 1}),
     "many rows": (3, 500, 500, 2, 1, 16, {"causal": 1, "slopes": 1}),    # more rows than one workgroup adds up
+    "documents of one": (2, 70, 70, 2, 1, 64, {"docs": 70, "causal": 1}),
     "few rows split": (1, 40, 2100, 2, 1, 64, {"causal": 1, "slopes": 1, "pad": 1}),
 }
 
@@ -214,6 +215,21 @@ def test_attention_slopes_gradient_of_bf16_is_exact_to_fp32(dev, name):
     want = attention_ref(q.float(), k.float(), v.float(), go.float(), **opt)
     out = A.score_attention(q, k, v, **{**opt, "slopes": opt["slopes"].requires_grad_(True)})
     check("dslopes", torch.autograd.grad(out, opt["slopes"], go)[0], want["dslopes"])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("S,H,Hk,D,cap", [(1, 2, 1, 64, 0.0), (70, 2, 1, 64, 0.0), (130, 4, 4, 192, 5.0), (200, 3, 1, 128, 0.0), (90, 2, 2, 256, 3.0), (40, 2, 1, 24, 0.0)])
+def test_rows_that_see_one_key_have_no_gradient_behind_the_softmax(dev, dtype, S, H, Hk, D, cap):
+    """P = 1 whatever the score is: the output is the value itself and dq, dk and dslopes are 0, not what rounding leaves of dP - delta."""
+    from transfusion_amd import attention_ops as A
+    g = gen(S + D)
+    q, k, v, go = (torch.randn(2, S, h, D, generator=g).to(dtype).to(dev).requires_grad_(True) for h in (H, Hk, Hk, H))
+    sl = torch.ones(H, device=dev, requires_grad=True)
+    doc = torch.arange(S, dtype=torch.int32, device=dev).expand(2, -1).contiguous()
+    out = A.score_attention(q, k, v, softcap=cap, slopes=sl, causal=True, q_doc=doc, k_doc=doc)
+    assert torch.equal(out, v.repeat_interleave(H // Hk, dim=2))
+    dq, dk, dsl = torch.autograd.grad(out, (q, k, sl), go.detach())
+    assert not dq.any() and not dk.any() and not dsl.any()
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])

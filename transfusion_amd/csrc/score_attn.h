@@ -59,20 +59,6 @@ __device__ __forceinline__ void landed(SFrag<false>& f) { asm volatile("" : "+v"
 __device__ __forceinline__ void landed(SFrag<true>& f) { asm volatile("" : "+v"(f.a), "+v"(f.b)); }
 __device__ __forceinline__ void landed(float& x) { asm volatile("" : "+v"(x)); }
 __device__ __forceinline__ void landed(int& x) { asm volatile("" : "+v"(x)); }
-template <bool F32> __device__ __forceinline__ float frag_dot(const SFrag<F32>& x, const SFrag<F32>& y) {
-  float s = 0.f;
-  if constexpr (F32) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s += x.a[e] * y.a[e] + x.b[e] * y.b[e];
-  } else {
-    float a[8], b[8];
-    unpack8(x.v, a);
-    unpack8(y.v, b);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s += a[e] * b[e];
-  }
-  return s;
-}
 
 // ---- the change of a score, in the log2 domain ----
 struct SMod {

@@ -6,8 +6,8 @@
 //
 // Bound by the registers: accumulators and row operands leave room for one wave a SIMD from 96 channels (dk / dv) or 192 (dq) on, so the products,
 // the exponentials and the barriers of a tile follow each other more than they overlap (dk / dv at 128 channels: matrix pipe busy 31 % of the
-// time, vector pipe 25 %).  4 x 4096 causal, 8 heads of 128: 575 us = 600 TFLOP/s (five products credited, seven computed); 4 x 2048, 16 heads of
-// 64: 298 us = 575; 32 x 708, 4 heads of 192: 276 us = 445.  Two forms that were no faster: a tile shared by two waves of a SIMD, P handed over
+// time, vector pipe 25 %).  4 x 4096 causal, 8 heads of 128: 547 us = 628 TFLOP/s (five products credited, seven computed); 4 x 2048, 16 heads of
+// 64: 277 us = 620; 32 x 708, 4 heads of 192: 272 us = 454.  Two forms that were no faster: a tile shared by two waves of a SIMD, P handed over
 // through LDS (the first size 606 us where this form took 603), and the next tile's scores formed under this one's products (spilled).
 #include "score_attn.h"
 
@@ -92,19 +92,27 @@ __global__ __launch_bounds__(256, dq_wgs(F32, HDP)) void score_dq_kernel(const T
   const char* qrow = qbase + (long long)ic * a.q_ss * G::ESZ;
   SFrag<F32> qf[REREAD ? 1 : G::KS], dof[REREAD ? 1 : G::KS];
   const char* drow = (const char*)a.dout + ((long long)b * a.do_sb + (long long)ic * a.do_ss + (long long)head * a.do_sh) * G::ESZ;
+  // delta by the matrix instructions that form dP, from the diagonal of dO O^T: a row that sees one key (o = v) gets dP - delta = 0 exactly
   float delta = 0.f;
   {
+    f32x16 dd;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dd[r] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < G::KS; ++ks) {
       const SFrag<F32> d = gfrag<F32>(drow, ks, h, a.D, live);
-      delta += frag_dot<F32>(d, gfrag<F32>((const char*)a.out + orow * G::ESZ, ks, h, a.D, live));
-      if (!F32 && a.out_lo != nullptr) delta += frag_dot<F32>(d, gfrag<F32>((const char*)a.out_lo + orow * G::ESZ, ks, h, a.D, live));
+      dd = smma<F32>(gfrag<F32>((const char*)a.out + orow * G::ESZ, ks, h, a.D, live), d, dd);
+      if (!F32 && a.out_lo != nullptr) dd = smma<F32>(gfrag<F32>((const char*)a.out_lo + orow * G::ESZ, ks, h, a.D, live), d, dd);
       if constexpr (!REREAD) {
         qf[ks] = gfrag<F32>(qrow, ks, h, a.D, live);
         dof[ks] = d;
       }
       if (F32 && HDP > 128) asm volatile("" ::: "memory");        // (a few loads at a time: the rows of O are not to lie in registers as a whole)
     }
+    // element (r & 3) + 8 (r >> 2) + 4 h of column lane & 31
+    const int c = lane & 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) delta = h == ((c >> 2) & 1) && r == ((c & 3) | (c >> 3) << 2) ? dd[r] : delta;
     delta += __shfl_xor(delta, 32, 64);
   }
   auto qx = [&](auto I) { if constexpr (REREAD) return gfrag<F32>(qrow, I, h, a.D, live); else return qf[I]; };
@@ -350,15 +358,12 @@ __global__ __launch_bounds__(256, dkv_wgs(F32, HDP, PART)) void score_dkv_kernel
           u32x4 ls[4];                      // register 4 g + e is query 8 g + 4 h + e
           const unsigned sa = stat0 + buf * 512 + hf * 128;
           static_for<4>([&](auto I) { ls[I] = rd128_asm<32 * I>(sa); });
-          if constexpr (DK) {               // dP - delta: the product starts at -delta
-            u32x4 de[4];
-            static_for<4>([&](auto I) { de[I] = rd128_asm<256 + 32 * I>(sa); });
-            static_for<4>([&](auto I) {
-              lgkm_wait<0>(de[I]);
+          u32x4 de[4];
+          if constexpr (DK) {               // (dP starts at 0 and delta comes off behind it, as in score_dq_kernel)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) dp[4 * I + e] = -f_of(de[I][e]);
-            });
+            for (int r = 0; r < 16; ++r) dp[r] = 0.f;
             mul_rows2<F32, HDP, PR::HALF>(fq, kx, vx, st, dp);
+            static_for<4>([&](auto I) { de[I] = rd128_asm<256 + 32 * I>(sa); });
           } else mul_rows<F32, HDP>(fq, kx, st);
           unsigned bits = 0xffffffffu;
           if (!full_t) {
@@ -370,7 +375,7 @@ __global__ __launch_bounds__(256, dkv_wgs(F32, HDP, PART)) void score_dkv_kernel
             }
             bits >>= 4 * h;
           }
-          static_for<4>([&](auto I) { lgkm_wait<0>(ls[I]); });
+          static_for<4>([&](auto I) { lgkm_wait<0>(ls[I]); if constexpr (DK) lgkm_wait<0>(de[I]); });
           const float pd = (float)(p0 + i0 + 4 * h - j), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
           SPack<F32> pp[1], ps[1];
           const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
@@ -383,7 +388,7 @@ __global__ __launch_bounds__(256, dkv_wgs(F32, HDP, PART)) void score_dkv_kernel
               pr = fast_exp2(x - f_of(ls[r >> 2][r & 3]));
               if (!FULL) pr = (bits >> q) & 1u ? pr : 0.f;
               if constexpr (DK) {
-                ds = pr * dp[r];
+                ds = pr * (dp[r] - f_of(de[r >> 2][r & 3]));
                 if (CAP) ds *= fmaf(t * t, ncap, 1.0f);
                 if (!FULL) ds = (bits >> q) & 1u ? ds : 0.f;        // (a hidden pair's product may not be finite)
               }
