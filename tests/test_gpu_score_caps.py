@@ -1,0 +1,64 @@
+"""Caps of every accepted size in attention with changed scores: a capped score may be off by a part of ITSELF, whatever the cap is, in every
+kernel (few rows, prompt, both backward kernels) and beside scores of any size."""
+import pytest
+import torch
+
+from operator_refs import check
+from score_bounds import attention_bounds
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs an MI355X")
+    from transfusion_amd import _lib
+    _lib.load()
+    return torch.device("cuda:0")
+
+
+def inputs(seed, B, Sq, Sk, H, Hk, D, dtype):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(B, s, h, D, generator=g).to(dtype) for s, h in ((Sq, H), (Sk, Hk), (Sk, Hk), (Sq, H))]
+
+
+def compare(dev, tensors, **opt):
+    from transfusion_amd import attention_ops as A
+    q, k, v, go = (t.to(dev) for t in tensors)
+    want = attention_bounds(q, k, v, go, **opt)
+    opt = {n: x.to(dev) if isinstance(x, torch.Tensor) else x for n, x in opt.items()}
+    with torch.no_grad():
+        check("inference", A.score_attention(q, k, v, **opt), want["out"])
+    q, k, v = (t.requires_grad_(True) for t in (q, k, v))
+    out = A.score_attention(q, k, v, **opt)
+    check("out", out, want["out"])
+    for n, gr in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), go)):
+        check(n, gr, want[n])
+
+
+SHAPES = [(1, 1, 77, 1, 1, 64), (2, 1, 300, 4, 2, 64), (2, 4, 513, 8, 1, 128), (1, 3, 260, 2, 2, 256),       # few rows
+          (1, 70, 70, 2, 1, 64), (1, 200, 333, 2, 2, 192)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cap", [1e-10, 1e-3, 1.0, 30.0, 1e3, 1e4, 1e6, 1e8, 1e10])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_every_cap(dev, shape, cap, dtype):
+    compare(dev, inputs(sum(shape), *shape, dtype), softcap=cap, causal=True)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cap", [1e3, 1e6])
+@pytest.mark.parametrize("shape", [(1, 4, 128, 2, 1, 64), (1, 96, 96, 2, 2, 64), (1, 160, 160, 2, 1, 128)])
+@pytest.mark.parametrize("kind", ["query", "hidden key"])
+def test_scores_beside_much_larger_ones(dev, kind, shape, cap, dtype):
+    """One query whose scores reach the cap, or a last key that only the last query sees and whose scores do: the other rows of the tile keep
+    their own precision."""
+    t = inputs(sum(shape) + 1, *shape, dtype)
+    if kind == "query":
+        t[0][:, 1] *= cap
+    else:
+        t[1][:, -1] *= cap
+    compare(dev, t, softcap=cap, causal=True)

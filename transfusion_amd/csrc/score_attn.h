@@ -65,14 +65,10 @@ struct SMod {
   float sc;          // no cap: scale * log2 e;  cap: 2 log2 e * scale / cap (the exponent of the tanh)
   float capl;        // cap * log2 e, or 0
   float slope2;      // slope * log2 e
-  float small;       // cap: scores (before the scale) up to this size take the polynomial below
+  float zs, zlim;    // cap: scores (before the scale, times zs) up to zlim take the polynomial below
+  float small;       // zlim where zs is 1, else -1
   float c0, c1, c2, c3;
 };
-template <bool F32> __device__ __forceinline__ float tanh_of(float y2) {       // y2 = 2 log2(e) y
-  if constexpr (F32) return tanhf(y2 * 0.34657359027997264f);
-  // 1 - 2 / (1 + e^2y): absolute error ~1e-7 (the bf16 product's own error is larger); +-inf give +-1, no NaN in between
-  return 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + fast_exp2(y2));
-}
 __device__ __forceinline__ float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
 __device__ __forceinline__ SMod smod(const TfScoreAttnArgs& a, int head) {
   SMod m;
@@ -80,22 +76,33 @@ __device__ __forceinline__ SMod smod(const TfScoreAttnArgs& a, int head) {
   m.sc = uniform(a.softcap > 0.f ? 2.f * LOG2E * a.scale / a.softcap : a.scale * LOG2E);
   m.slope2 = a.slopes != nullptr ? uniform(a.slopes[head] * LOG2E) : 0.f;
   // tanh y = y (1 - y^2 / 3 ...) for |y| <= 1/2: a least-maximum fit of degree 3 in y^2, relative error 5e-7.  Scores are mostly far below the
-  // cap, and five multiplications cost less than half of an exponential and a reciprocal (two quarter-rate instructions).
-  const float g = a.softcap > 0.f ? a.scale / a.softcap : 0.f, g2 = g * g;
-  m.small = uniform(g2 > 0.f && g2 < 1e12f ? fminf(0.5f / fabsf(g), 1e15f) : -1.f);       // (beyond, powers leave fp32's range)
-  m.c0 = uniform(0.99999946f * m.capl * g);
-  m.c1 = uniform(-0.33326318f * m.capl * g * g2);
-  m.c2 = uniform(0.13190297f * m.capl * g * g2 * g2);
-  m.c3 = uniform(-0.04440223f * m.capl * g * g2 * g2 * g2);
+  // cap, and five multiplications cost less than half of an exponential and a reciprocal (two quarter-rate instructions).  The powers of y / score
+  // are folded into the coefficients; where they leave fp32's range the polynomial takes s * sc = 2 log2(e) y instead of s.
+  const float g = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
+  const bool in = g * g > 0.f && g * g < 1e12f;
+  const float y = in ? g : 0.5f / LOG2E, y2 = y * y;
+  m.zs = uniform(in ? 1.f : m.sc);
+  m.zlim = uniform(fminf(0.5f / fabsf(y), 1e15f));
+  m.small = in ? m.zlim : -1.f;
+  m.c0 = uniform(0.99999946f * m.capl * y);
+  m.c1 = uniform(-0.33326318f * m.capl * y * y2);
+  m.c2 = uniform(0.13190297f * m.capl * y * y2 * y2);
+  m.c3 = uniform(-0.04440223f * m.capl * y * y2 * y2 * y2);
   return m;
 }
-// cap * tanh(scale s / cap) in the log2 domain
-template <bool F32> __device__ __forceinline__ float capped_exact(const SMod& m, float s) { return m.capl * tanh_of<F32>(s * m.sc); }
 __device__ __forceinline__ float capped_poly(float s, float c0, float c1, float c2, float c3) {
   const float u = s * s;
   return s * fmaf(u, fmaf(u, fmaf(u, c3, c2), c1), c0);
 }
-// are all scores of a tile small enough for the polynomial?  (wave-uniform; a NaN stays one either way)
+// cap * tanh(scale s / cap) in the log2 domain, to 2^-20 of its value.  1 - 2 / (1 + e^2y) alone (+-inf give +-1, no NaN in between) is off by 2e-7
+// whatever its size: under a cap of 1e6 that is 0.2 of every score, however small.
+template <bool F32> __device__ __forceinline__ float capped(const SMod& m, float s) {
+  if constexpr (F32) return m.capl * tanhf(s * m.sc * 0.34657359027997264f);
+  const float z = s * m.zs, low = capped_poly(z, m.c0, m.c1, m.c2, m.c3);
+  const float high = m.capl * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + fast_exp2(s * m.sc)));
+  return fabsf(z) <= m.zlim ? low : high;
+}
+// are all scores of a tile small enough for the polynomial as they stand?  (wave-uniform; a NaN stays one either way)
 template <bool F32, int N> __device__ __forceinline__ bool all_small(const SMod& m, const f32x16 (&st)[N]) {
   if (F32) return false;                  // (fp32: the polynomial's 5e-7 would show)
   float top = 0.f;
@@ -104,6 +111,27 @@ template <bool F32, int N> __device__ __forceinline__ bool all_small(const SMod&
 #pragma unroll
     for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(st[k][r]));
   return __all(top <= m.small);
+}
+// score by score, in place
+template <bool F32> __device__ __forceinline__ void cap_each(const SMod& m, f32x16& st) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) st[r] = capped<F32>(m, st[r]);
+}
+// the capped scores of a forward's tile, in place.  (One branch that rewrites the scores; as two arms the forms cost a second set of registers.)
+template <bool F32, int N> __device__ __forceinline__ void cap_scores(const SMod& m, f32x16 (&st)[N]) {
+  float c0 = m.c0, c1 = m.c1, c2 = m.c2, c3 = m.c3;
+  if (!all_small<F32, N>(m, st)) {        // the polynomial below becomes the identity
+#pragma unroll
+    for (int k = 0; k < N; ++k) cap_each<F32>(m, st[k]);
+    c0 = 1.f;
+    c1 = c2 = c3 = 0.f;
+  }
+  if (!F32) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st[k][r] = capped_poly(st[k][r], c0, c1, c2, c3);
+  }
 }
 // position of query 0 (bounded so that sums with a query number stay in 32 bits) and the prefix length of sample b
 __device__ __forceinline__ int q_pos0(const TfScoreAttnArgs& a, int b) {
@@ -516,7 +544,7 @@ __device__ __forceinline__ int key_end(const TfScoreAttnArgs& a, int p0, int pfx
 __device__ __forceinline__ unsigned low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 // body(FULL, CAP, SLP) with the flags (all uniform over the wave) as compile-time constants: the loops over a tile's scores stay free of
-// branches and of registers that only one of their forms needs.  CAP: 0 none, 1 tanh, 2 its polynomial
+// branches and of registers that only one of their forms needs.  CAP: 0 none, 1 tanh (bf16: cap_each has done it), 2 its polynomial
 template <class F> __device__ __forceinline__ void by_flags(bool full, int cap, bool slp, F&& body) {
   auto three = [&](auto FULL, auto CAP) { if (slp) body(FULL, CAP, std::true_type{}); else body(FULL, CAP, std::false_type{}); };
   auto two = [&](auto FULL) {

@@ -179,13 +179,13 @@ __global__ __launch_bounds__(256, dq_wgs(F32, HDP)) void score_dq_kernel(const T
         const float pd = (float)(qr.p - kv0 - 4 * h), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
         SPack<F32> pk[1];
         const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
-        const int cap = m.capl == 0.f ? 0 : all_small<F32, 1>(m, raw) ? 2 : 1;
+        const int cap = m.capl == 0.f ? 0 : !F32 && a.dslopes == nullptr && all_small<F32, 1>(m, raw) ? 2 : 1;
         auto form = [&](auto FULL, auto CAP, auto SLP, auto SUMS) {
           f32x4 t4 = {0, 0, 0, 0};
+          if (!F32 && CAP == 1) cap_each<SUMS>(m, st);            // (sums: the cap as exactly as fp32 has it)
           auto one = [&](int r) {
             const int j = (r & 3) + 8 * (r >> 2);
-            // (sums: the cap as exactly as fp32 has it)
-            float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? capped_exact<F32 || SUMS>(m, st[r]) : st[r] * m.sc, x = t;
+            float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? (F32 ? capped<true>(m, st[r]) : st[r]) : st[r] * m.sc, x = t;
             const float dist = SLP ? fabsf(pd - (float)j) : 0.f;
             if (SLP) x -= m.slope2 * dist;
             float pr = fast_exp2(x - lse);
@@ -381,9 +381,10 @@ __global__ __launch_bounds__(256, dkv_wgs(F32, HDP, PART)) void score_dkv_kernel
           const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
           const int cap = m.capl == 0.f ? 0 : all_small<F32, 1>(m, raw) ? 2 : 1;
           by_flags(full_t, cap, m.slope2 != 0.f, [&](auto FULL, auto CAP, auto SLP) {
+            if (!F32 && CAP == 1) cap_each<false>(m, st);
             auto one = [&](int r, float& pr, float& ds) {
               const int q = (r & 3) + 8 * (r >> 2);
-              float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? capped_exact<F32>(m, st[r]) : st[r] * m.sc, x = t;
+              float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? (F32 ? capped<true>(m, st[r]) : st[r]) : st[r] * m.sc, x = t;
               if (SLP) x -= m.slope2 * fabsf(pd + (float)q);
               pr = fast_exp2(x - f_of(ls[r >> 2][r & 3]));
               if (!FULL) pr = (bits >> q) & 1u ? pr : 0.f;

@@ -90,23 +90,7 @@ __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <
       auto qx = [&](auto I) { if constexpr (REREAD) return gfrag<F32>(qrow, I, h, a.D, live); else return qf[I]; };
       mul_rows2<F32, HDP, 32 * G::STR>(f0, qx, qx, st[0], st[1]);
       // each change is a branch that rewrites the scores in place (uniform; as two arms of one branch they cost a second set of registers)
-      if (m.capl != 0.f) {
-        float c0 = m.c0, c1 = m.c1, c2 = m.c2, c3 = m.c3;
-        if (!all_small<F32, 2>(m, st)) {  // exactly, and the polynomial below becomes the identity
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) st[kb][r] = capped_exact<F32>(m, st[kb][r]);
-          c0 = 1.f;
-          c1 = c2 = c3 = 0.f;
-        }
-        if (!F32) {
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) st[kb][r] = capped_poly(st[kb][r], c0, c1, c2, c3);
-        }
-      }
+      if (m.capl != 0.f) cap_scores<F32, 2>(m, st);
       if (scaled) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -224,8 +208,7 @@ __device__ __forceinline__ FewRows few_rows(const TfScoreAttnArgs& a, int b, int
 template <bool F32, bool DOC> __device__ __forceinline__ void few_change(const TfScoreAttnArgs& a, const FewRows& w, const SMod& m, int p0, int kv0, int kd, int h,
                                                                          f32x16& st) {
   if (m.capl != 0.f) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) st[r] = capped_exact<F32>(m, st[r]);
+    cap_scores<F32, 1>(m, reinterpret_cast<f32x16 (&)[1]>(st));
   } else {
 #pragma unroll
     for (int r = 0; r < 16; ++r) st[r] *= m.sc;
