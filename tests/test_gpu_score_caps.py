@@ -62,3 +62,13 @@ def test_scores_beside_much_larger_ones(dev, kind, shape, cap, dtype):
     else:
         t[1][:, -1] *= cap
     compare(dev, t, softcap=cap, causal=True)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("scale,cap", [(9e5, 1.0), (1e10, 1e5), (1e10, 1e10), (1e10, 1e-10), (-9e5, 1.0), (1e-3, 1e10), (1e-20, 1e10), (0.0, 1.0)])
+@pytest.mark.parametrize("shape", [(1, 2, 90, 2, 1, 64), (1, 70, 70, 2, 1, 64)])
+def test_scores_of_zero(dev, shape, scale, cap, dtype):
+    """A query of zeros attends every key alike, whatever scale and cap make of other scores."""
+    t = inputs(sum(shape) + 2, *shape, dtype)
+    t[0].zero_()
+    compare(dev, t, scale=scale, softcap=cap)

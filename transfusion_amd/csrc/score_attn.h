@@ -79,10 +79,11 @@ __device__ __forceinline__ SMod smod(const TfScoreAttnArgs& a, int head) {
   // cap, and five multiplications cost less than half of an exponential and a reciprocal (two quarter-rate instructions).  The powers of y / score
   // are folded into the coefficients; where they leave fp32's range the polynomial takes s * sc = 2 log2(e) y instead of s.
   const float g = a.softcap > 0.f ? a.scale / a.softcap : 0.f;
-  const bool in = g * g > 0.f && g * g < 1e12f;
+  const float last = fabsf(m.capl * g * (g * g) * (g * g) * (g * g));
+  const bool in = last > 1e-36f && last < 1e36f;         // (a coefficient that is infinite makes a NaN of a score of 0)
   const float y = in ? g : 0.5f / LOG2E, y2 = y * y;
   m.zs = uniform(in ? 1.f : m.sc);
-  m.zlim = uniform(fminf(0.5f / fabsf(y), 1e15f));
+  m.zlim = uniform(0.5f / fabsf(y));
   m.small = in ? m.zlim : -1.f;
   m.c0 = uniform(0.99999946f * m.capl * y);
   m.c1 = uniform(-0.33326318f * m.capl * y * y2);
