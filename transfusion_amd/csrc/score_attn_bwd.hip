@@ -470,7 +470,7 @@ __device__ __forceinline__ double slope_rows(const Finish& f, unsigned head, uns
       d += (double)r[2 * rows];
       ed += (double)r[3 * rows];
     }
-    if (p > 0.0) s -= (ed - e * d / p) / p;               // -cov(e, dist); a row that sees nothing has none
+    if (p != 0.0) s -= (ed - e * d / p) / p;              // -cov(e, dist); a row that sees nothing has none (its p is 0), a NaN goes on
   }
   return block_sum(s, tid);
 }
