@@ -556,14 +556,20 @@ template <class F> __device__ __forceinline__ void by_flags(bool full, int cap, 
   if (full) two(std::true_type{}); else two(std::false_type{});
 }
 
-// dynamic LDS beyond the default limit is granted per device
-template <class K> void allow_lds(K kern, size_t bytes) {
+// Launches KERN with `bytes` of dynamic LDS (always the same for a kernel).  What lies beyond the default limit is granted per kernel and device: a
+// kernel is a template value here, so each has a flag of its own (a flag per type would be shared by all widths), set once the runtime has agreed.
+template <auto KERN, class... Args> int launch_lds(int blocks, size_t bytes, hipStream_t st, Args... args) {
   static std::atomic<unsigned long long> done{0};
   int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev > 63) dev = 0;
-  if (done.load(std::memory_order_relaxed) >> dev & 1ull) return;
-  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return (int)e;
+  if (dev > 63 || !(done.load(std::memory_order_relaxed) >> dev & 1ull)) {
+    e = hipFuncSetAttribute((const void*)KERN, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != hipSuccess) return (int)e;
+    if (dev <= 63) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  hipLaunchKernelGGL(KERN, dim3(blocks), dim3(256), bytes, st, args...);
+  return (int)hipGetLastError();
 }
 
 // Ways to split the `units` (tiles of keys or queries) of a loop that `blocks` workgroups run.  bf16: until two workgroups a CU are there, `least` units

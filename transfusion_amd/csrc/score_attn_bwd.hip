@@ -533,25 +533,27 @@ template <bool F32, int HDP> int launch_bwd(const TfScoreAttnArgs* a, hipStream_
   const double fl = 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D;
   const BwdPlan pl = bwd_plan(a, a->dslopes != nullptr);
   const bool doc = a->k_doc != nullptr;
-  auto go = [&](auto kern, int blocks, size_t lds) {
-    allow_lds(kern, lds);
-    hipLaunchKernelGGL(kern, dim3(blocks), dim3(256), lds, st, *a, pl);
-  };
+  int rc = 0;
   if (const int blocks = a->B * a->H * pl.nqb * pl.sq; blocks > 0) {
     TfTraceScope tr(F32 ? "score_dq_kernel<fp32>" : "score_dq_kernel<bf16>", st, 1.5 * fl);
     constexpr size_t lds = Pair<F32, HDP, dq_wgs(F32, HDP)>::LDS;
-    doc ? go(score_dq_kernel<F32, HDP, true>, blocks, lds) : go(score_dq_kernel<F32, HDP, false>, blocks, lds);
+    rc = doc ? launch_lds<score_dq_kernel<F32, HDP, true>>(blocks, lds, st, *a, pl) : launch_lds<score_dq_kernel<F32, HDP, false>>(blocks, lds, st, *a, pl);
   }
+  if (rc != 0) return rc;
   if (const int blocks = a->B * a->Hk * pl.nkb * pl.sg * pl.sk; blocks > 0) {
     TfTraceScope tr(F32 ? "score_dkv_kernel<fp32>" : "score_dkv_kernel<bf16>", st, 2.0 * fl);
     auto part = [&](auto which) {
       constexpr int PART = decltype(which)::value;
       constexpr size_t lds = Pair<F32, HDP, dkv_wgs(F32, HDP, PART)>::LDS;
-      doc ? go(score_dkv_kernel<F32, HDP, PART, true>, blocks, lds) : go(score_dkv_kernel<F32, HDP, PART, false>, blocks, lds);
+      return doc ? launch_lds<score_dkv_kernel<F32, HDP, PART, true>>(blocks, lds, st, *a, pl) : launch_lds<score_dkv_kernel<F32, HDP, PART, false>>(blocks, lds, st, *a, pl);
     };
-    if constexpr (HDP <= (F32 ? 128 : 192)) part(std::integral_constant<int, 2>{});
-    else { part(std::integral_constant<int, 0>{}); part(std::integral_constant<int, 1>{}); }
+    if constexpr (HDP <= (F32 ? 128 : 192)) rc = part(std::integral_constant<int, 2>{});
+    else {
+      rc = part(std::integral_constant<int, 0>{});
+      if (rc == 0) rc = part(std::integral_constant<int, 1>{});
+    }
   }
+  if (rc != 0) return rc;
   const int ns = pl.sg * pl.sk;
   Finish f{};
   f.rows = (const float*)a->work + pl.o_rows;

@@ -564,24 +564,25 @@ template <bool F32, int HDP> int launch_fwd(const TfScoreAttnArgs* a, hipStream_
   const FwdPlan f = fwd_plan(a);
   const bool doc = a->k_doc != nullptr;
   const double fl = 4.0 * a->B * a->H * (double)a->Sq * a->Sk * a->D;
+  int rc;
   if (f.few) {
     TfTraceScope tr(F32 ? "score_few32_kernel" : "score_few16_kernel", st, fl);
-    const size_t join = (128 * (size_t)HDP + 256) * 4;
-    auto go = [&](auto kern, size_t lds) {
-      allow_lds(kern, std::max(lds, join));
-      hipLaunchKernelGGL(kern, dim3(a->B * a->Hk * f.nsplit), dim3(256), std::max(lds, join), st, *a, f.nsplit);
-    };
-    if constexpr (F32) doc ? go(score_few32_kernel<HDP, true>, 0) : go(score_few32_kernel<HDP, false>, 0);
-    else doc ? go(score_few16_kernel<HDP, true>, 8 * SDma<false, HDP, 32, 1>::BYTES) : go(score_few16_kernel<HDP, false>, 8 * SDma<false, HDP, 32, 1>::BYTES);
+    const int blocks = a->B * a->Hk * f.nsplit;
+    constexpr size_t join = (128 * (size_t)HDP + 256) * 4;
+    if constexpr (F32) {
+      rc = doc ? launch_lds<score_few32_kernel<HDP, true>>(blocks, join, st, *a, f.nsplit) : launch_lds<score_few32_kernel<HDP, false>>(blocks, join, st, *a, f.nsplit);
+    } else {
+      constexpr size_t lds = std::max<size_t>(8 * SDma<false, HDP, 32, 1>::BYTES, join);
+      rc = doc ? launch_lds<score_few16_kernel<HDP, true>>(blocks, lds, st, *a, f.nsplit) : launch_lds<score_few16_kernel<HDP, false>>(blocks, lds, st, *a, f.nsplit);
+    }
   } else {
     TfTraceScope tr(F32 ? "score_fwd_kernel<fp32>" : "score_fwd_kernel<bf16>", st, fl);
-    auto go = [&](auto kern) {
-      const size_t lds = 2 * SDma<F32, HDP, 64, 4>::BYTES + 640;
-      allow_lds(kern, lds);
-      hipLaunchKernelGGL(kern, dim3(a->B * a->H * f.nqb * f.nsplit), dim3(256), lds, st, *a, f.nqb, f.nsplit, f.split_tiles);
-    };
-    doc ? go(score_fwd_kernel<F32, HDP, true>) : go(score_fwd_kernel<F32, HDP, false>);
+    const int blocks = a->B * a->H * f.nqb * f.nsplit;
+    constexpr size_t lds = 2 * SDma<F32, HDP, 64, 4>::BYTES + 640;
+    rc = doc ? launch_lds<score_fwd_kernel<F32, HDP, true>>(blocks, lds, st, *a, f.nqb, f.nsplit, f.split_tiles)
+             : launch_lds<score_fwd_kernel<F32, HDP, false>>(blocks, lds, st, *a, f.nqb, f.nsplit, f.split_tiles);
   }
+  if (rc != 0) return rc;
   if (f.nsplit > 1) {
     TfTraceScope tr("score_join_kernel", st);
     const unsigned rows = (unsigned)((long long)a->B * a->H * a->Sq);
