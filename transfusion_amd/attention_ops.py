@@ -12,6 +12,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from transfusion_amd import _lib as L
 from transfusion_amd import ops
@@ -69,6 +70,12 @@ def _keep(dev, *tensors):
     for t in tensors:
         if t is not None and t.numel():
             t.record_stream(st)
+
+
+def _recorded(*tensors):
+    """Does autograd have to see this call?  (inside a forward-mode level always: it refuses dual tensors there, which have no tangent behind a
+    kernel called directly)"""
+    return forward_ad._current_level >= 0 or torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors])
 
 
 # ------------------------------------------------------------------------------------------------------
@@ -167,7 +174,7 @@ def rotary(q, k, pos, plan: RotaryPlan):
     if tuple(pos.shape) not in ((B, S, len(plan.axes)), (S, len(plan.axes))):
         raise L.TfError(f"rotary: positions {tuple(pos.shape)}, expected {(B, S, len(plan.axes))} or {(S, len(plan.axes))}")
     pos = pos.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if _recorded(q, k):
         return _RotaryFn.apply(q, k, pos, plan)
     qo, ko = _rotary_call(q, k, pos, plan, False)
     return qo if k is None else (qo, ko)
@@ -280,6 +287,6 @@ def score_attention(q, k, v, scale: float = None, softcap: float = 0.0, slopes=N
     if q_doc is not None:
         q_doc = _ints("score_attention q_doc", q_doc, (B, Sq), dev)
         k_doc = _ints("score_attention k_doc", k_doc, (B, Sk), dev)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, slopes)):
+    if _recorded(q, k, v, slopes):
         return _ScoreAttnFn.apply(q, k, v, slopes, scale, softcap, int(bool(causal)), prefix, q_start, q_doc, k_doc)
     return _score_fwd(q, k, v, (scale, softcap, slopes, int(bool(causal)), prefix, q_start, q_doc, k_doc), False)[3]
