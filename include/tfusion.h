@@ -622,7 +622,8 @@ typedef struct TfScoreAttnArgs {
   const void* k; long long k_sb, k_ss, k_sh;     // [B, Sk, Hk, D]
   const void* v; long long v_sb, v_ss, v_sh;     // [B, Sk, Hk, D]
   void* out;                                     // [B, Sq, H, D] contiguous
-  float* lse;                                    // [B, H, Sq] fp32 (log2 domain; +inf for rows without keys), or null without a backward
+  float* lse;                                    // [B, H, Sq] fp32, or null without a backward: log2 domain, distances counted from the position in
+                                                 // [0, Sk) nearest to p (the rest is common to the row's keys); +inf for rows without keys
   int B, Sq, Sk, H, Hk, D; int is_f32;
   float scale, softcap;
   const float* slopes;                           // [H] fp32 or null

@@ -1,4 +1,5 @@
-"""The gradient of learned slopes where values are not finite: what a row sees reaches it, what is hidden does not."""
+"""Slopes of attention with changed scores: gradients where values are not finite (what a row sees reaches them, what is hidden does not), and
+queries far from the keys."""
 import math
 
 import pytest
@@ -62,3 +63,18 @@ def test_what_is_hidden_does_not(dev, Sq, Sk, dtype):
         t[dead < 0] = x
     for n, got in zip(("out", "dq", "dk", "dv", "dslopes"), gradients(q, k, v, go, sl, **opt)):
         check(n, got, want[n])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", [(4, 2, 300, 4, 2, 64), (4, 70, 70, 2, 1, 32), (4, 140, 200, 2, 2, 128)])
+def test_queries_far_from_the_keys(dev, shape, causal, dtype):
+    """Queries behind the last key, before the first, across either end, up to the largest number: a shift of all distances of a row changes neither
+    the softmax nor a gradient, so no precision may be lost to it."""
+    q, k, v, go, sl = inputs(sum(shape) + 3, *shape, dtype, dev)
+    for starts in ((1000000, 200, 2 ** 31 - 1, 65), (-3, -1000000, -2 ** 31, 280)):
+        start = torch.tensor(starts, dtype=torch.int32, device=dev)
+        opt = {"causal": causal, "q_start": start, "softcap": 20.0}
+        want = attention_bounds(q, k, v, go, slopes=sl, **opt)
+        for n, got in zip(("out", "dq", "dk", "dv", "dslopes"), gradients(q, k, v, go, sl, **opt)):
+            check(f"{n} {starts}", got, want[n])

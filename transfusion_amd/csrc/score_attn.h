@@ -121,7 +121,7 @@ template <bool F32> __device__ __forceinline__ void cap_each(const SMod& m, f32x
 // the capped scores of a forward's tile, in place.  (One branch that rewrites the scores; as two arms the forms cost a second set of registers.)
 template <bool F32, int N> __device__ __forceinline__ void cap_scores(const SMod& m, f32x16 (&st)[N]) {
   float c0 = m.c0, c1 = m.c1, c2 = m.c2, c3 = m.c3;
-  if (!all_small<F32, N>(m, st)) {        // the polynomial below becomes the identity
+  if (__builtin_expect(!all_small<F32, N>(m, st), F32)) {         // the polynomial below becomes the identity
 #pragma unroll
     for (int k = 0; k < N; ++k) cap_each<F32>(m, st[k]);
     c0 = 1.f;
@@ -528,12 +528,16 @@ __device__ __forceinline__ void order_blocks(int nb, int per, bool uneven, int& 
   block = blockIdx.x / n;
   group = n / per % 8 == 0 ? (8 * (y / per) + (g & 7)) * per + y % per : n % 8 == 0 ? (g & 7) * (n >> 3) + y : g;
 }
+// Distances count from the position among the keys that is nearest to the query's: the rest is the same for every key of the row, so the softmax
+// and its gradients do not know it, and beside it -- 2^20 positions times a slope -- fp32 would lose the scores (slope 0.5 at position 10^6 on 300
+// keys: probabilities off by several per cent).  The stored log-sum-exp lacks it as well.
+__device__ __forceinline__ int near_pos(const TfScoreAttnArgs& a, int p) { return min(max(p, 0), a.Sk - 1); }
 // what a query row may see: everything below follows from these
-struct QRow { int p, lim, lim_lo, lim_hi; };       // position; last visible key of this row, of the wave's first row, of its last
+struct QRow { int p, lim, lim_lo, lim_hi; };       // position for distances; last visible key of this row, of the wave's first row, of its last
 __device__ __forceinline__ QRow q_row(const TfScoreAttnArgs& a, int p0, int pfx, int w0, int i) {
   QRow q;
-  q.p = p0 + i;
-  q.lim = a.causal ? min(max(q.p, pfx - 1), a.Sk - 1) : a.Sk - 1;
+  q.p = near_pos(a, p0 + i);
+  q.lim = a.causal ? min(max(p0 + i, pfx - 1), a.Sk - 1) : a.Sk - 1;
   q.lim_lo = a.causal ? min(max(p0 + w0, pfx - 1), a.Sk - 1) : a.Sk - 1;
   q.lim_hi = a.causal ? min(max(p0 + min(w0 + 31, a.Sq - 1), pfx - 1), a.Sk - 1) : a.Sk - 1;
   return q;

@@ -382,11 +382,17 @@ __global__ __launch_bounds__(256, dkv_wgs(F32, HDP, PART)) void score_dkv_kernel
           const int cap = m.capl == 0.f ? 0 : all_small<F32, 1>(m, raw) ? 2 : 1;
           by_flags(full_t, cap, m.slope2 != 0.f, [&](auto FULL, auto CAP, auto SLP) {
             if (!F32 && CAP == 1) cap_each<false>(m, st);
+            float ll[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              // (the bias goes to the log-sum-exp; distances: near_pos of the query, less the key)
+              ll[r] = f_of(ls[r >> 2][r & 3]);
+              if (SLP) ll[r] = fmaf(m.slope2, fabsf(__builtin_amdgcn_fmed3f(pd + (float)((r & 3) + 8 * (r >> 2)), (float)-j, (float)(a.Sk - 1 - j))), ll[r]);
+            }
             auto one = [&](int r, float& pr, float& ds) {
               const int q = (r & 3) + 8 * (r >> 2);
-              float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? (F32 ? capped<true>(m, st[r]) : st[r]) : st[r] * m.sc, x = t;
-              if (SLP) x -= m.slope2 * fabsf(pd + (float)q);
-              pr = fast_exp2(x - f_of(ls[r >> 2][r & 3]));
+              const float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? (F32 ? capped<true>(m, st[r]) : st[r]) : st[r] * m.sc;
+              pr = fast_exp2(t - ll[r]);
               if (!FULL) pr = (bits >> q) & 1u ? pr : 0.f;
               if constexpr (DK) {
                 ds = pr * (dp[r] - f_of(de[r >> 2][r & 3]));

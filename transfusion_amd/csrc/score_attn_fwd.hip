@@ -190,7 +190,7 @@ __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <
 // the four waves walks key tiles of its own (32 keys) and the workgroup's keys are a range of the sample's (the launcher splits the keys
 // until the chip is full).  bf16: no barrier in the loop -- a wave waits for its own transfers by count: K(t + 1) is under way from the
 // moment S(t) has been read, V(t + 1) from the end of PV(t), so one tile is always in flight.  The waves' parts are joined in LDS.
-struct FewRows { int i, head, lim, qd; bool ok, live; float slope2; };
+struct FewRows { int i, head, p, lim, qd; bool ok, live; float slope2; };       // (p: see near_pos)
 __device__ __forceinline__ FewRows few_rows(const TfScoreAttnArgs& a, int b, int kvh, int p0, int pfx, int lane) {
   FewRows w;
   const int G = a.H / a.Hk, r = lane & 31;
@@ -200,12 +200,13 @@ __device__ __forceinline__ FewRows few_rows(const TfScoreAttnArgs& a, int b, int
   w.head = kvh * G + rc % G;
   w.qd = a.k_doc != nullptr ? a.q_doc[(size_t)b * a.Sq + w.i] : 0;
   w.live = w.ok && w.qd >= 0;
+  w.p = near_pos(a, p0 + w.i);
   w.lim = a.causal ? min(max(p0 + w.i, pfx - 1), a.Sk - 1) : a.Sk - 1;
   w.slope2 = a.slopes != nullptr ? a.slopes[w.head] * LOG2E : 0.f;
   return w;
 }
 // the changed and masked scores of a 32-key tile (kd: document of key kv0 + (lane & 31))
-template <bool F32, bool DOC> __device__ __forceinline__ void few_change(const TfScoreAttnArgs& a, const FewRows& w, const SMod& m, int p0, int kv0, int kd, int h,
+template <bool F32, bool DOC> __device__ __forceinline__ void few_change(const TfScoreAttnArgs& a, const FewRows& w, const SMod& m, int kv0, int kd, int h,
                                                                          f32x16& st) {
   if (m.capl != 0.f) {
     cap_scores<F32, 1>(m, reinterpret_cast<f32x16 (&)[1]>(st));
@@ -214,7 +215,7 @@ template <bool F32, bool DOC> __device__ __forceinline__ void few_change(const T
     for (int r = 0; r < 16; ++r) st[r] *= m.sc;
   }
   if (a.slopes != nullptr) {
-    const float pd = (float)(p0 + w.i - kv0 - 4 * h);
+    const float pd = (float)(w.p - kv0 - 4 * h);
 #pragma unroll
     for (int r = 0; r < 16; ++r) st[r] -= w.slope2 * fabsf(pd - (float)((r & 3) + 8 * (r >> 2)));
   }
@@ -387,7 +388,7 @@ __global__ __launch_bounds__(256, (HDP <= 128 ? 2 : 1)) void score_few16_kernel(
     for (int r = 0; r < 16; ++r) st[r] = 0.f;
     mul_rows<false, HDP>(fk, [&](auto I) { return qf[I]; }, st);
     if (tn >= 0) issue(kdma, kbase, krb, tn, kt, neg_t);
-    few_change<false, DOC>(a, w, m, p0, t * 32, kd, h, st);
+    few_change<false, DOC>(a, w, m, t * 32, kd, h, st);
     few_softmax<G::DB>(st, m_run, l_run, o);
     SPack<false> pk[1];
 #pragma unroll
@@ -447,7 +448,7 @@ __global__ __launch_bounds__(256, 1) void score_few32_kernel(const TfScoreAttnAr
       if constexpr (REREAD) st = smma<true>(x, gfrag<true>(qrow, ks, h, a.D, w.live), st);
       else st = smma<true>(x, qf[ks], st);
     }
-    few_change<true, DOC>(a, w, m, p0, kv0, kd, h, st);
+    few_change<true, DOC>(a, w, m, kv0, kd, h, st);
     few_softmax<DB>(st, m_run, l_run, o);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
