@@ -72,3 +72,46 @@ def test_scores_of_zero(dev, shape, scale, cap, dtype):
     t = inputs(sum(shape) + 2, *shape, dtype)
     t[0].zero_()
     compare(dev, t, scale=scale, softcap=cap)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cap", [0.0, 1e10])
+@pytest.mark.parametrize("slope", [None, 0.0, 0.25, 1e9])
+@pytest.mark.parametrize("scale", [1e4, 1e7, 1e10])
+@pytest.mark.parametrize("shape", [(1, 2, 90, 2, 1, 64), (2, 70, 70, 2, 1, 64), (1, 150, 333, 2, 2, 128)])
+def test_scores_beyond_all_measure(dev, shape, scale, slope, cap, dtype):
+    """Scores far apart: every row takes one value whole, and its gradient is that value's.  Query i is the unit vector of channel i % D, the keys hold
+    whole numbers, so that scores are exact up to the scale's (and the cap's) rounding, and the winner is ahead by more than that."""
+    from transfusion_amd import attention_ops as A
+    if cap and 256 * scale > cap:
+        pytest.skip("the cap makes ties of all of them")
+    q, k, v, go = inputs(sum(shape) + 4, *shape, dtype)
+    B, Sq, Sk, H, Hk, D = shape
+    q.zero_()
+    q[:, torch.arange(Sq), :, torch.arange(Sq) % D] = 1.0
+    g = torch.Generator().manual_seed(5)
+    k = torch.stack([torch.randperm(Sk, generator=g) for _ in range(B * Hk * D)]).view(B, Hk, D, Sk).permute(0, 3, 1, 2).remainder(256).to(dtype)
+    slopes = None if slope is None else torch.full((H,), slope)
+    t = torch.einsum("bihd,bjhd->bhij", q.double(), k.double().repeat_interleave(H // Hk, dim=2)) * scale
+    t = cap * torch.tanh(t / cap) if cap else t
+    p, j = torch.arange(Sk - Sq, Sk), torch.arange(Sk)
+    if slope:
+        t = t - slope * (p[:, None] - j).abs().double()
+    t = t.masked_fill(j > p[:, None], -float("inf"))
+    top = t.topk(2, dim=-1)
+    sure = (top.values[..., 0] - top.values[..., 1]) > 64 + 2.0 ** -18 * top.values.abs().amax(-1)       # [B, H, Sq]
+    assert sure.float().mean() > 0.3
+    go = go * sure.permute(0, 2, 1)[..., None]
+    best = top.indices[..., 0]
+    vh = v.repeat_interleave(H // Hk, dim=2).permute(0, 2, 1, 3)
+    want = torch.gather(vh, 2, best[..., None].expand(-1, -1, -1, D))
+    dv = torch.zeros(B, H, Sk, D, dtype=torch.float64).scatter_add_(2, best[..., None].expand(-1, -1, -1, D), go.double().permute(0, 2, 1, 3))
+    dv = dv.view(B, Hk, H // Hk, Sk, D).sum(2).permute(0, 2, 1, 3)
+    leaves = [x.to(dev).requires_grad_(True) for x in (q, k, v)]
+    out = A.score_attention(*leaves, scale=scale, softcap=cap, slopes=None if slopes is None else slopes.to(dev), causal=True)
+    got = out.detach().cpu().permute(0, 2, 1, 3)
+    assert torch.isfinite(got).all() and torch.equal(got[sure], want[sure])
+    dq, dk, dv_ = torch.autograd.grad(out, leaves, go.to(dev))
+    assert torch.isfinite(dq).all() and torch.isfinite(dk).all()
+    # sums of up to Sq H / Hk terms in fp32, rounded to the type
+    check("dv", dv_, (dv, dv.abs() * 2.0 ** (-8 if dtype == BF else -24) + Sq * H * 2.0 ** -24 * 8 + 1e-30))

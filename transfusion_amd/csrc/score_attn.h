@@ -113,10 +113,22 @@ template <bool F32, int N> __device__ __forceinline__ bool all_small(const SMod&
     for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(st[k][r]));
   return __all(top <= m.small);
 }
-// score by score, in place
+// Beyond this size (log2 domain) what rounding takes from a score is more than a small part of its probability: there every kernel forms the same
+// rounded score and only then takes the row's maximum or log-sum-exp off it.  Left to itself, a product that rides in an FMA with the maximum is not
+// rounded: at 10^10 the largest score then lies up to 512 beyond "itself", an infinity or a zero in place of a one.
+constexpr float S_BIG = 4096.f;
+__device__ __forceinline__ bool big(float x) { return fabsf(x) > S_BIG && fabsf(x) < INFINITY; }
+// (no FMA across it)
+__device__ __forceinline__ float rounded(float x) { asm("" : "+v"(x)); return x; }
+// score by score, in place: capped, or only scaled
 template <bool F32> __device__ __forceinline__ void cap_each(const SMod& m, f32x16& st) {
+  if (m.capl != 0.f) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) st[r] = capped<F32>(m, st[r]);
+    for (int r = 0; r < 16; ++r) st[r] = rounded(capped<F32>(m, st[r]));
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st[r] = rounded(st[r] * m.sc);
+  }
 }
 // the capped scores of a forward's tile, in place.  (One branch that rewrites the scores; as two arms the forms cost a second set of registers.)
 template <bool F32, int N> __device__ __forceinline__ void cap_scores(const SMod& m, f32x16 (&st)[N]) {
@@ -549,12 +561,12 @@ __device__ __forceinline__ int key_end(const TfScoreAttnArgs& a, int p0, int pfx
 __device__ __forceinline__ unsigned low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 // body(FULL, CAP, SLP) with the flags (all uniform over the wave) as compile-time constants: the loops over a tile's scores stay free of
-// branches and of registers that only one of their forms needs.  CAP: 0 none, 1 tanh (bf16: cap_each has done it), 2 its polynomial
+// branches and of registers that only one of their forms needs.  CAP: 0 none, 1 score by score (cap_each), 2 the cap's polynomial
 template <class F> __device__ __forceinline__ void by_flags(bool full, int cap, bool slp, F&& body) {
   auto three = [&](auto FULL, auto CAP) { if (slp) body(FULL, CAP, std::true_type{}); else body(FULL, CAP, std::false_type{}); };
   auto two = [&](auto FULL) {
     if (cap == 2) three(FULL, std::integral_constant<int, 2>{});
-    else if (cap == 1) three(FULL, std::integral_constant<int, 1>{});
+    else if (__builtin_expect(cap == 1, false)) three(FULL, std::integral_constant<int, 1>{});
     else three(FULL, std::integral_constant<int, 0>{});
   };
   if (full) two(std::true_type{}); else two(std::false_type{});

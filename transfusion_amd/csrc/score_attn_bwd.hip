@@ -45,7 +45,7 @@ template <bool F32, int DB> __device__ __forceinline__ void store_grad(void* out
 struct BwdPlan {
   unsigned chunks;                       // of the slopes' rows
   int nqb, nkb, sq, sg, sk;              // splits of dq (keys); of dk / dv: groups of heads x ranges of queries
-  size_t o_dk, o_dv, o_rows, o_part, floats;
+  size_t o_dk, o_dv, o_rows, o_part, o_far, floats;       // o_far: a word per 32 queries of a head, is one of their log-sum-exps big (see S_BIG)
 };
 
 // ================================================================================================
@@ -118,6 +118,8 @@ __global__ __launch_bounds__(256, dq_wgs(F32, HDP)) void score_dq_kernel(const T
   auto qx = [&](auto I) { if constexpr (REREAD) return gfrag<F32>(qrow, I, h, a.D, live); else return qf[I]; };
   auto dx = [&](auto I) { if constexpr (REREAD) return gfrag<F32>(drow, I, h, a.D, live); else return dof[I]; };
   float lse = live ? a.lse[row] : INFINITY;
+  const bool far = !F32 && __any(big(lse));              // (uniform: see S_BIG)
+  const int mode = far ? 1 : m.capl == 0.f ? 0 : F32 || a.dslopes != nullptr ? 1 : 2;        // by_flags' CAP; 2: where a tile's scores allow it
   landed(lse);
   landed(delta);
   if constexpr (!REREAD) {
@@ -179,15 +181,18 @@ __global__ __launch_bounds__(256, dq_wgs(F32, HDP)) void score_dq_kernel(const T
         const float pd = (float)(qr.p - kv0 - 4 * h), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
         SPack<F32> pk[1];
         const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
-        const int cap = m.capl == 0.f ? 0 : !F32 && a.dslopes == nullptr && all_small<F32, 1>(m, raw) ? 2 : 1;
+        const int cap = mode == 2 && !all_small<F32, 1>(m, raw) ? 1 : mode;
         auto form = [&](auto FULL, auto CAP, auto SLP, auto SUMS) {
           f32x4 t4 = {0, 0, 0, 0};
-          if (!F32 && CAP == 1) cap_each<SUMS>(m, st);            // (sums: the cap as exactly as fp32 has it)
+          if (!F32 && CAP == 1) {
+            if (SUMS && !far) cap_each<SUMS>(m, st);              // (sums: the cap as exactly as fp32 has it)
+            else cap_each<false>(m, st);
+          }
           auto one = [&](int r) {
             const int j = (r & 3) + 8 * (r >> 2);
-            float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? (F32 ? capped<true>(m, st[r]) : st[r]) : st[r] * m.sc, x = t;
+            float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? (F32 ? rounded(capped<true>(m, st[r])) : st[r]) : F32 ? rounded(st[r] * m.sc) : st[r] * m.sc, x = t;
             const float dist = SLP ? fabsf(pd - (float)j) : 0.f;
-            if (SLP) x -= m.slope2 * dist;
+            if (SLP) x = fmaf(-m.slope2, dist, x);
             float pr = fast_exp2(x - lse);
             x = pr * (dp[r] - delta);
             if (!FULL) x = (bits >> j) & 1u ? x : 0.f;
@@ -198,7 +203,7 @@ __global__ __launch_bounds__(256, dq_wgs(F32, HDP)) void score_dq_kernel(const T
               t4[2] = fmaf(pr, dist, t4[2]);
               t4[3] = fmaf(x, dist, t4[3]);
             }
-            return CAP ? x * fmaf(t * t, ncap, 1.0f) : x;           // the cap's derivative: 1 - (t / cap)^2
+            return CAP ? x * fmaf(t * ncap, t, 1.0f) : x;           // the cap's derivative: 1 - (t / cap)^2
           };
 #pragma unroll
           for (int r = 0; r < 16; r += 2) {
@@ -236,6 +241,7 @@ __global__ __launch_bounds__(256, dq_wgs(F32, HDP)) void score_dq_kernel(const T
     }
   }
   if (i < a.Sq && h == 0 && split == 0) a.delta[row] = delta;
+  if (!F32 && lane == 0 && split == 0) ((int*)a.work + pl.o_far)[((size_t)bh * pl.nqb + qb) * 4 + wave] = far;
 #pragma unroll
   for (int d = 0; d < G::DB; ++d)
 #pragma unroll
@@ -313,6 +319,14 @@ __global__ __launch_bounds__(256, dkv_wgs(F32, HDP, PART)) void score_dkv_kernel
     const char* xbase = wave < 2 ? (const char*)a.q + ((long long)b * a.q_sb + (long long)head * a.q_sh) * G::ESZ
                                  : (const char*)a.dout + ((long long)b * a.do_sb + (long long)head * a.do_sh) * G::ESZ;
     const long long row0 = ((long long)b * a.H + head) * a.Sq;
+    bool far = false;                     // as in score_dq_kernel, for all queries of the head
+    if (!F32) {
+      const int* flag = (const int*)a.work + pl.o_far + ((size_t)b * a.H + head) * pl.nqb * 4;
+      int any = 0;
+      for (int x = lane; x < pl.nqb * 4; x += 64) any |= flag[x];
+      far = __any(any != 0);
+    }
+    const int mode = far ? 1 : m.capl == 0.f ? 0 : F32 ? 1 : 2;
     auto fetch = [&](int buf) {           // the pair in walk.s, its rows' statistics (waves 0 and 1) and documents, 4 bytes a lane
       const int i0 = walk.s * 32;
       // (queries behind the last are hidden by number, whatever document they show)
@@ -379,24 +393,28 @@ __global__ __launch_bounds__(256, dkv_wgs(F32, HDP, PART)) void score_dkv_kernel
           const float pd = (float)(p0 + i0 + 4 * h - j), ncap = m.capl != 0.f ? -1.0f / (m.capl * m.capl) : 0.f;
           SPack<F32> pp[1], ps[1];
           const f32x16 (&raw)[1] = reinterpret_cast<const f32x16 (&)[1]>(st);
-          const int cap = m.capl == 0.f ? 0 : all_small<F32, 1>(m, raw) ? 2 : 1;
+          const int cap = mode == 2 && !all_small<F32, 1>(m, raw) ? 1 : mode;
           by_flags(full_t, cap, m.slope2 != 0.f, [&](auto FULL, auto CAP, auto SLP) {
             if (!F32 && CAP == 1) cap_each<false>(m, st);
+            // distances: near_pos of the query, less the key
+            auto bias = [&](int r, float x, float slope2) {
+              return fmaf(slope2, fabsf(__builtin_amdgcn_fmed3f(pd + (float)((r & 3) + 8 * (r >> 2)), (float)-j, (float)(a.Sk - 1 - j))), x);
+            };
+            constexpr bool EACH = F32 || CAP == 1;       // the bias comes off the score, as in the forward; else it goes to the log-sum-exp (fewer registers)
             float ll[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              // (the bias goes to the log-sum-exp; distances: near_pos of the query, less the key)
               ll[r] = f_of(ls[r >> 2][r & 3]);
-              if (SLP) ll[r] = fmaf(m.slope2, fabsf(__builtin_amdgcn_fmed3f(pd + (float)((r & 3) + 8 * (r >> 2)), (float)-j, (float)(a.Sk - 1 - j))), ll[r]);
+              if (SLP && !EACH) ll[r] = bias(r, ll[r], m.slope2);
             }
             auto one = [&](int r, float& pr, float& ds) {
               const int q = (r & 3) + 8 * (r >> 2);
-              const float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? (F32 ? capped<true>(m, st[r]) : st[r]) : st[r] * m.sc;
-              pr = fast_exp2(t - ll[r]);
+              const float t = CAP == 2 ? capped_poly(st[r], m.c0, m.c1, m.c2, m.c3) : CAP == 1 ? (F32 ? rounded(capped<true>(m, st[r])) : st[r]) : F32 ? rounded(st[r] * m.sc) : st[r] * m.sc;
+              pr = fast_exp2((SLP && EACH ? bias(r, t, -m.slope2) : t) - ll[r]);
               if (!FULL) pr = (bits >> q) & 1u ? pr : 0.f;
               if constexpr (DK) {
                 ds = pr * (dp[r] - f_of(de[r >> 2][r & 3]));
-                if (CAP) ds *= fmaf(t * t, ncap, 1.0f);
+                if (CAP) ds *= fmaf(t * ncap, t, 1.0f);
                 if (!FULL) ds = (bits >> q) & 1u ? ds : 0.f;        // (a hidden pair's product may not be finite)
               }
             };
@@ -531,7 +549,8 @@ BwdPlan bwd_plan(const TfScoreAttnArgs* a, bool slopes) {
   p.o_rows = p.o_dv + (ns > 1 ? ns * nk : 0);
   p.chunks = slopes ? (unsigned)(((long long)a->B * a->Sq + SLOPE_CHUNK - 1) / SLOPE_CHUNK) : 0;
   p.o_part = (p.o_rows + (slopes ? 4 * (size_t)p.sq * a->B * a->H * a->Sq : 0) + 1) / 2 * 2;
-  p.floats = p.o_part + (p.chunks > 1 ? 2 * (size_t)p.chunks * a->H : 0);
+  p.o_far = p.o_part + (p.chunks > 1 ? 2 * (size_t)p.chunks * a->H : 0);
+  p.floats = p.o_far + (a->is_f32 ? 0 : 4 * (size_t)a->B * a->H * p.nqb);
   return p;
 }
 

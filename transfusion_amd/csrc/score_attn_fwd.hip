@@ -10,7 +10,9 @@ namespace {
 // Bound by the vector work between the two products (exponential, cap, masks, rounding) and by the barriers: matrix and vector pipes are busy 45 % of
 // the time each at 128 channels, 42 and 70 % at 64.  A causal prompt of 16384 tokens, 8 heads of 128: 620 us = 890 TFLOP/s (a large library product
 // reaches 1215 on this card); 4 x 2048, 16 heads of 64: 83 us = 830 TFLOP/s; 32 x 708, 4 heads of 192: 64 us = 770 TFLOP/s.
-template <bool F32, int HDP, bool DOC>
+// RIDE (bf16, no cap, no slopes, a scale > 0, which leaves the order of the scores as it is): the scale rides in the exponent's FMA, until a row's maximum
+// is large (see S_BIG).  A form of its own: the same switch in the loop of all forms cost a causal prompt of 16384 with slopes, 8 heads of 128, 2 % (600 -> 612 us).
+template <bool F32, int HDP, bool DOC, bool RIDE>
 __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <= 96 ? 3 : HDP <= (F32 ? 64 : 192) ? 2 : 1)) void score_fwd_kernel(const TfScoreAttnArgs a, int nqb, int nsplit, int split_tiles) {
   using G = SGeo<F32, HDP>;
   using Dma = SDma<F32, HDP, 64, 4>;
@@ -50,9 +52,8 @@ __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
   float m_run = S_NEG, l_run = 0.f;
-  // without a cap or a slope, and where it does not turn the order of the scores round, the scale rides in the exponent's FMA
-  const bool scaled = m.capl == 0.f && (m.slope2 != 0.f || !(m.sc > 0.f));
-  const float scf = m.capl != 0.f || scaled ? 1.0f : m.sc;
+  bool scaled = !RIDE && m.capl == 0.f;
+  float scf = RIDE ? m.sc : 1.0f;
   const SAddr<F32, HDP> f0(lds_addr_of(smem), lane);
   const Dma dma(wave, lane, krb, a.D);
   int t = walk.first(split * split_tiles, dsh, wave, lane);
@@ -90,14 +91,14 @@ __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <
       auto qx = [&](auto I) { if constexpr (REREAD) return gfrag<F32>(qrow, I, h, a.D, live); else return qf[I]; };
       mul_rows2<F32, HDP, 32 * G::STR>(f0, qx, qx, st[0], st[1]);
       // each change is a branch that rewrites the scores in place (uniform; as two arms of one branch they cost a second set of registers)
-      if (m.capl != 0.f) cap_scores<F32, 2>(m, st);
+      if (!RIDE && m.capl != 0.f) cap_scores<F32, 2>(m, st);
       if (scaled) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) st[kb][r] *= m.sc;
       }
-      if (m.slope2 != 0.f) {
+      if (!RIDE && m.slope2 != 0.f) {
         const float pd = (float)(row_.p - kv0 - 4 * h);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -134,6 +135,14 @@ __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <
         for (int d = 0; d < G::DB; ++d)
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+        if (RIDE && scf != 1.0f && __any(big(m_run) && m_run != S_NEG)) {        // from here on the scores are rounded first
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[kb][r] *= scf;
+          scaled = true;
+          scf = 1.0f;
+        }
       }
       float ps0 = 0.f, ps1 = 0.f;
 #pragma unroll
@@ -217,7 +226,7 @@ template <bool F32, bool DOC> __device__ __forceinline__ void few_change(const T
   if (a.slopes != nullptr) {
     const float pd = (float)(w.p - kv0 - 4 * h);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) st[r] -= w.slope2 * fabsf(pd - (float)((r & 3) + 8 * (r >> 2)));
+    for (int r = 0; r < 16; ++r) st[r] = fmaf(-w.slope2, fabsf(pd - (float)((r & 3) + 8 * (r >> 2))), st[r]);
   }
   unsigned bits = low_bits(w.lim - kv0 + 1);
   if (DOC) bits &= (unsigned)doc_bits(w.qd, kd);
@@ -230,6 +239,7 @@ template <bool F32, bool DOC> __device__ __forceinline__ void few_change(const T
 }
 // one step of the running softmax over a 32-key tile: st becomes the probabilities
 template <int DB> __device__ __forceinline__ void few_softmax(f32x16& st, float& m_run, float& l_run, f32x16 (&o)[DB]) {
+#pragma clang fp contract(off)            // (the maximum comes off the rounded score: see S_BIG)
   float mx = -INFINITY;
 #pragma unroll
   for (int r = 0; r < 16; ++r) mx = fmaxf(mx, st[r]);
@@ -580,8 +590,12 @@ template <bool F32, int HDP> int launch_fwd(const TfScoreAttnArgs* a, hipStream_
     TfTraceScope tr(F32 ? "score_fwd_kernel<fp32>" : "score_fwd_kernel<bf16>", st, fl);
     const int blocks = a->B * a->H * f.nqb * f.nsplit;
     constexpr size_t lds = 2 * SDma<F32, HDP, 64, 4>::BYTES + 640;
-    rc = doc ? launch_lds<score_fwd_kernel<F32, HDP, true>>(blocks, lds, st, *a, f.nqb, f.nsplit, f.split_tiles)
-             : launch_lds<score_fwd_kernel<F32, HDP, false>>(blocks, lds, st, *a, f.nqb, f.nsplit, f.split_tiles);
+    auto go = [&](auto ride) {
+      return doc ? launch_lds<score_fwd_kernel<F32, HDP, true, decltype(ride)::value>>(blocks, lds, st, *a, f.nqb, f.nsplit, f.split_tiles)
+                 : launch_lds<score_fwd_kernel<F32, HDP, false, decltype(ride)::value>>(blocks, lds, st, *a, f.nqb, f.nsplit, f.split_tiles);
+    };
+    if constexpr (F32) rc = go(std::false_type{});
+    else rc = a->softcap == 0.f && a->slopes == nullptr && a->scale > 0.f ? go(std::true_type{}) : go(std::false_type{});
   }
   if (rc != 0) return rc;
   if (f.nsplit > 1) {
