@@ -616,7 +616,8 @@ int tf_rotary(const TfRotaryArgs* a, tf_stream_t s);
  * q_doc[b][i] == k_doc[b][j] >= 0 (when given) and (causal == 0 or j <= p or j < prefix[b]).  Rows without keys give zeros and take no
  * gradient.  What rows of negative documents, and keys beyond the causal horizon of the last query, hold in memory is never used (NaN
  * included).  H % Hk == 0: H / Hk consecutive heads share a key / value head.  D <= 256, D % 8 == 0; bf16 or fp32; every
- * pointer and stride a multiple of 16 bytes.  Statistics and sums are fp32; results do not depend on the launch's timing. */
+ * pointer and stride a multiple of 16 bytes.  Statistics and sums are fp32; results do not depend on the launch's timing.  The backward
+ * forms the probabilities again from the fp32 log-sum-exp: all of a row's together may be off by its last place, 2^-24 of the largest score. */
 typedef struct TfScoreAttnArgs {
   const void* q; long long q_sb, q_ss, q_sh;     // [B, Sq, H, D], strides of batch, token and head in elements, channels contiguous
   const void* k; long long k_sb, k_ss, k_sh;     // [B, Sk, Hk, D]

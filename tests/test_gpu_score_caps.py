@@ -115,3 +115,11 @@ def test_scores_beyond_all_measure(dev, shape, scale, slope, cap, dtype):
     assert torch.isfinite(dq).all() and torch.isfinite(dk).all()
     # sums of up to Sq H / Hk terms in fp32, rounded to the type
     check("dv", dv_, (dv, dv.abs() * 2.0 ** (-8 if dtype == BF else -24) + Sq * H * 2.0 ** -24 * 8 + 1e-30))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-6, 3.0])
+@pytest.mark.parametrize("shape", [(1, 3, 130, 2, 1, 64), (2, 150, 150, 2, 1, 96)])
+def test_scales_of_either_sign(dev, shape, scale, cap, dtype):
+    compare(dev, inputs(sum(shape) + 6, *shape, dtype), scale=scale, softcap=cap, causal=True)

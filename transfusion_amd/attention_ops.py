@@ -253,7 +253,9 @@ def score_attention(q, k, v, scale: float = None, softcap: float = 0.0, slopes=N
 
     unless it is hidden: ``causal`` hides j > p except the first ``prefix[b]`` keys (int32 [B]); ``q_doc`` / ``k_doc`` (int32 [B, Sq] /
     [B, Sk]) hide keys of other documents, and a negative document is padding: attends nothing, is attended by nobody, and whatever its
-    rows hold is not used.  A query that sees nothing gets zeros.  ``scale`` (within 1e10) defaults to 1 / sqrt(D);
+    rows hold is not used.  A query that sees nothing gets zeros.  (A NaN or an infinity in a key or value that some query sees may reach queries beside
+    it that do not: 0 times it is not 0.)  Scores are fp32 numbers: what lies below the last place of a row's largest one, 2^-24 of it, is lost to
+    probabilities and gradients.  ``scale`` (within 1e10) defaults to 1 / sqrt(D);
     ``softcap`` is 0 or between 1e-10 and 1e10.  D <= 256, a multiple of 8."""
     _heads("score_attention q", q)
     _heads("score_attention k", k, like=q)

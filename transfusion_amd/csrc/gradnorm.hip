@@ -7,7 +7,7 @@
 // Every workgroup of the first pass writes ONE 64-bit partial; every workgroup of the second pass adds all of them up again in index
 // order (a few thousand values from L2) -- no atomics, no counter to reset, the same bits on every run and rank, and no third launch.
 // Squares are accumulated in 64 bits: neither the length of the sum nor a gradient beyond 2^64 costs anything, and the kernel stays
-// bound by its loads (fp64 FMA runs at an eighth of the rate the loads could feed).
+// bound by its loads: they bring 1.2 (fp32) to 2.4 (bf16) elements a picosecond, the card forms up to 39 fp64 FMAs in that time.
 #include "tf_common.h"
 #include "tf_kernels.h"
 #include <algorithm>

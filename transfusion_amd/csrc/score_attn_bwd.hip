@@ -6,8 +6,8 @@
 //
 // Bound by the registers: accumulators and row operands leave room for one wave a SIMD from 96 channels (dk / dv) or 192 (dq) on, so the products,
 // the exponentials and the barriers of a tile follow each other more than they overlap (dk / dv at 128 channels: matrix pipe busy 31 % of the
-// time, vector pipe 25 %).  4 x 4096 causal, 8 heads of 128: 547 us = 628 TFLOP/s (five products credited, seven computed); 4 x 2048, 16 heads of
-// 64: 277 us = 620; 32 x 708, 4 heads of 192: 272 us = 454.  Two forms that were no faster: a tile shared by two waves of a SIMD, P handed over
+// time, vector pipe 25 %).  4 x 4096 causal, 8 heads of 128: 557 us = 617 TFLOP/s (five products credited, seven computed); 4 x 2048, 16 heads of
+// 64: 281 us = 611; 32 x 708, 4 heads of 192: 274 us = 450.  Two forms that were no faster: a tile shared by two waves of a SIMD, P handed over
 // through LDS (the first size 606 us where this form took 603), and the next tile's scores formed under this one's products (spilled).
 #include "score_attn.h"
 

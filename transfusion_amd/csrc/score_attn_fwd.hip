@@ -195,9 +195,9 @@ __global__ __launch_bounds__(256, (!F32 && HDP <= 64 && !DOC ? 4 : !F32 && HDP <
 // ================================================================================================
 // forward of few rows (single tokens): Sq * H / Hk <= 32
 // ================================================================================================
-// Bound by the bytes of K and V: 4 x 16411 keys, 16 heads of 128 on 4, take 28 us = 4.75 TB/s (a large copy reaches 4.87).  The rows of all heads that share a key head are one 32-column tile, so every key is read once; each of
-// the four waves walks key tiles of its own (32 keys) and the workgroup's keys are a range of the sample's (the launcher splits the keys
-// until the chip is full).  bf16: no barrier in the loop -- a wave waits for its own transfers by count: K(t + 1) is under way from the
+// Bound by the bytes of K and V: 4 x 16411 keys, 16 heads of 128 on 4, take 25.7 us = 5.2 TB/s (a large copy reaches 4.87), and 4 us the join.  The
+// rows of all heads that share a key head are one 32-column tile, so every key is read once; each of the four waves walks key tiles of its own
+// (32 keys) and the workgroup's keys are a range of the sample's (the launcher splits the keys until the chip is full).  bf16: no barrier in the loop -- a wave waits for its own transfers by count: K(t + 1) is under way from the
 // moment S(t) has been read, V(t + 1) from the end of PV(t), so one tile is always in flight.  The waves' parts are joined in LDS.
 struct FewRows { int i, head, p, lim, qd; bool ok, live; float slope2; };       // (p: see near_pos)
 __device__ __forceinline__ FewRows few_rows(const TfScoreAttnArgs& a, int b, int kvh, int p0, int pfx, int lane) {
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(256, (HDP <= 128 ? 2 : 1)) void score_few16_kernel(
 }
 
 // fp32: K fragments and V rows come straight from memory (V's are whole 128-byte lines a half-wave, the fp32 matrix instruction takes them
-// untransposed), so nothing is staged; many waves hide the latency
+// untransposed), so nothing is staged and a wave waits for its loads tile by tile: the same size takes 313 us = 0.86 TB/s
 template <int HDP, bool DOC>
 __global__ __launch_bounds__(256, 1) void score_few32_kernel(const TfScoreAttnArgs a, int nsplit) {
   constexpr int KS = HDP / 16, DB = HDP / 32;

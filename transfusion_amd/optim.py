@@ -42,7 +42,8 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0):
     all of them as a 0-d fp32 device tensor (no host synchronisation) and multiplies every gradient by ``min(1, max_norm / (norm + 1e-6))``
     in place.  ``max_norm=inf`` only measures.  ``norm_type``: 2 or inf.  Gradients are fp32 or bf16 tensors (mixed freely) on one device that
     fill their memory without gaps, in any order of their axes; a parameter listed twice counts once, parameters without a gradient are
-    skipped.  A norm that is not finite behaves as in torch: an infinite one zeroes what is finite, a NaN spreads."""
+    skipped, gradients of different parameters must not share memory.  A norm that is not finite behaves as in torch: an infinite one zeroes
+    what is finite, a NaN spreads."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     max_norm, norm_type = float(max_norm), float(norm_type)
